@@ -1,4 +1,4 @@
-"""ctypes bindings of the C ABIs declared in include/fa_b200.h, fa_b200_rows.h, fa_b200_hybrid.h and fa_b200_mixers.h.
+"""ctypes bindings of the C ABIs declared in include/fa_b200.h, fa_b200_rows.h, fa_b200_hybrid.h, fa_b200_mixers.h and fa_b200_kv8.h.
 
 The libraries are loaded from the package directory, each when an operator of it is first used.  There is no
 fallback: if a library is missing, the use of any of its operators raises, with the build command in the message.
@@ -132,9 +132,26 @@ MIXERS_SIGNATURES = {
     "fam_kv_prefill": (_i, [_vp] * 5 + [_i, _i, _i64, _i64, _i, _i, _i, _i, _f, _vp, _vp, _i64, _vp, _i64, _vp, _vp]),
 }
 
+# every symbol include/fa_b200_kv8.h declares
+class Kv8Cache(_c.Structure):
+    """FakCache"""
+    _fields_ = [("k", _vp), ("v", _vp), ("scale", _vp), ("pages", _i64), ("heads", _i), ("dim", _i), ("codes", _i), ("table", _vp), ("width", _i),
+                ("max_pages", _i)]
+
+
+_k8 = _c.POINTER(Kv8Cache)
+KV8_SIGNATURES = {
+    "fak_last_error": (_c.c_char_p, []),
+    "fak_status": (_i, [_vp, _c.POINTER(_i), _i]),
+    "fak_append_paged": (_i, [_k8, _vp, _vp, _i64, _i64, _i, _vp, _vp, _i, _i64, _vp]),
+    "fak_decode_workspace": (_sz, [_k8, _i, _i, _i, _i]),
+    "fak_decode_paged": (_i, [_k8, _vp, _vp, _vp, _i, _i, _i, _i, _f, _vp, _vp, _i, _i, _vp, _sz, _vp]),
+    "fak_evict_paged": (_i, [_k8, _vp, _vp, _i, _i, _vp, _i, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
+}
+
 _libs = {}
 _ABIS = {"attention": (SIGNATURES, "fa"), "rows": (ROWS_SIGNATURES, "far"), "hybrid": (HYBRID_SIGNATURES, "fah"),
-         "mixers": (MIXERS_SIGNATURES, "fam")}
+         "mixers": (MIXERS_SIGNATURES, "fam"), "kv8": (KV8_SIGNATURES, "fak")}
 
 
 def _open(path: str, signatures) -> ctypes.CDLL:

@@ -3,8 +3,8 @@
 `libfa_b200.so` (csrc/*.cu) holds the attention operators and the operators of the Qwen3-style decoder; the hybrid
 decoders share `libfa_b200_rows.so` (csrc/rows/*.cu, row-wise operators) and have their mixers in
 `libfa_b200_hybrid.so` (csrc/hybrid/*.cu: decayed linear attention, latent attention) and `libfa_b200_mixers.so`
-(csrc/mixers/*.cu: gated recurrences, chunked attention).  A process that serves one model builds and loads what that
-model needs.
+(csrc/mixers/*.cu: gated recurrences, chunked attention).  `libfa_b200_kv8.so` (csrc/kv8/*.cu) holds the operators on a paged cache in
+8 bits.  A process that serves one model builds and loads what that model needs.
 
     python -m flash_attn_v100_b200.build            # rebuild what is out of date, all libraries
     python -m flash_attn_v100_b200.build --force
@@ -48,7 +48,7 @@ LINK_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-Xcompil
 
 LIBRARIES = {"attention": (LIB_PATH, CSRC)}
 LIBRARIES.update({name: (os.path.join(PKG_DIR, f"libfa_b200_{name}.so"), os.path.join(CSRC, name))
-                  for name in ("rows", "hybrid", "mixers")})
+                  for name in ("rows", "hybrid", "mixers", "kv8")})
 
 
 def sources(library: str = "attention"):

@@ -1,0 +1,166 @@
+// New keys and values into the pages of the 8-bit cache.
+//
+// For each page, head and kind that gets rows: a = max |x| of the new rows, scale' = max(a / top, 2^-100, the scale before if the page has
+// rows already), code = round(x / scale').  Bound by HBM: a prompt's row of D values is read as 2 D bytes and written as D.  One warp takes a page of one head
+// and kind whole into registers (D bytes a lane), so the rows are read once; the largest magnitude is found on the 16-bit patterns two at a
+// time, where NaN is above infinity.
+#include "kv8.cuh"
+
+namespace fa {
+namespace kv8 {
+namespace {
+
+template <bool BF16>
+__device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b) {
+  if constexpr (BF16) {
+    a = __uint_as_float(w << 16);
+    b = __uint_as_float(w & 0xffff0000u);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<__half2*>(&w));
+    a = f.x;
+    b = f.y;
+  }
+}
+
+// `n` rows from `row` on (stride in elements) into the slots from `slot` on of one page.
+template <int D, bool E4M3, bool BF16>
+__device__ __forceinline__ void append_page(const AppendArgs& a, const uint16_t* row, int64_t stride, uint8_t* codes, float* scale, int slot, int n, int lane) {
+  constexpr int kLanes = D / 8;              // lanes of a row, 16 bytes each
+  constexpr int kRows = 32 / kLanes;         // rows of one load
+  constexpr int kLoads = kPage / kRows;
+  const int r0 = lane / kLanes, col = lane % kLanes;
+  uint4 x[kLoads];
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int r = i * kRows + r0;
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (r < n) x[i] = load_stream16(row + r * stride + col * 8);
+  }
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) most = __vmaxu2(most, w[j] & 0x7fff7fffu);
+  }
+  most = max(most & 0xffffu, most >> 16);
+  most = __reduce_max_sync(0xffffffffu, most);
+  float m, unused;
+  unpack2<BF16>(most, m, unused);
+  if (!(m <= 3.4028235e38f)) m = __int_as_float(0x7f800000);
+  const float before = slot > 0 ? *scale : 0.f;
+  const float made = fmaxf(fmaxf(__fmul_rn(m, (float)(1.0 / top_of(E4M3))), kLeastScale), before);
+  if (slot > 0 && made > before) {           // the page's earlier rows, again
+    const float ratio = __fdiv_rn(before, made);
+    uint32_t* old = reinterpret_cast<uint32_t*>(codes);
+    for (int i = lane; i < slot * (D / 4); i += 32) old[i] = recode4<E4M3>(old[i], ratio);
+  }
+  __syncwarp();
+  if (lane == 0) *scale = made;
+  const bool finite = made <= 3.4028235e38f;
+  const float inv = __frcp_rn(made);
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int r = i * kRows + r0;
+    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    uint32_t out[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float f[4];
+      unpack2<BF16>(w[2 * j], f[0], f[1]);
+      unpack2<BF16>(w[2 * j + 1], f[2], f[3]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = __fmul_rn(f[e], inv);
+      out[j] = finite ? encode4<E4M3>(f) : 0u;
+    }
+    if (r < n) *reinterpret_cast<uint2*>(codes + (slot + r) * D + col * 8) = make_uint2(out[0], out[1]);
+  }
+}
+
+// The sequence of packed token t: the last one with cu[b] <= t that is not empty.
+__device__ __forceinline__ int sequence_of(const int* cu, int batch, int64_t t) {
+  int lo = 0, hi = batch;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (cu[mid] <= t) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+constexpr int kWarps = 4;
+
+// A warp per window of tokens (packed prompts: 16, a decode step: 1), head and kind: it takes the pages that begin, for this call, in the window.
+template <int D, bool E4M3, bool BF16>
+__global__ void __launch_bounds__(kWarps * 32) append_kernel(const AppendArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int window = a.cu != nullptr ? kPage : 1;
+  const int heads = a.c.heads;
+  const int64_t job = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const int kind = (int)(job & 1);
+  const int h = (int)((job >> 1) % heads);
+  const int64_t first = (job >> 1) / heads * window;
+  if (first >= a.total) return;
+  // lane i < window: token first + i, and whether it is the first of a page's new rows
+  const int64_t t = first + lane;
+  int b = 0, slot = 0, n = 0;
+  int64_t end = 0;
+  bool leads = false;
+  if (lane < window && t < a.total) {
+    int64_t begin;
+    if (a.cu != nullptr) {
+      b = sequence_of(a.cu, a.batch, t);
+      begin = a.cu[b];
+      end = min((int64_t)a.cu[b + 1], a.total);
+    } else {
+      b = (int)t;
+      begin = t;
+      end = t + 1;
+    }
+    if (t >= begin && t < end && begin >= 0) {
+      const int64_t pos = (a.positions != nullptr ? a.positions[b] : 0) + (t - begin);
+      slot = (int)(pos & (kPage - 1));
+      leads = t == begin || slot == 0;
+      n = (int)min((int64_t)(kPage - slot), end - t);
+      const int64_t index = pos >> 4;
+      int id = -1;
+      if (pos >= 0 && index < a.c.max_pages) id = a.c.table[(int64_t)b * a.c.width + index];
+      if (leads && !page_ok(a.c, id)) {
+        atomicOr(a.c.status, kStatusBadPageId);
+        leads = false;
+      }
+      b = id;                                  // from here on: the page
+    }
+  }
+  const uint16_t* rows = static_cast<const uint16_t*>(kind ? a.v : a.k) + (int64_t)h * D;
+  const int64_t stride = kind ? a.v_stride : a.k_stride;
+  for (uint32_t todo = __ballot_sync(0xffffffffu, leads); todo; todo &= todo - 1) {
+    const int i = __ffs(todo) - 1;
+    const int page = __shfl_sync(0xffffffffu, b, i);
+    const int s = __shfl_sync(0xffffffffu, slot, i), count = __shfl_sync(0xffffffffu, n, i);
+    const int64_t at = (int64_t)page * heads + h;
+    append_page<D, E4M3, BF16>(a, rows + (first + i) * stride, stride, (kind ? a.c.v : a.c.k) + at * kPage * D, a.c.scale + at * 2 + kind, s, count, lane);
+  }
+}
+
+template <int D, bool E4M3>
+cudaError_t launch_append_d(const AppendArgs& a, bool bf16, cudaStream_t s) {
+  const int window = a.cu != nullptr ? kPage : 1;
+  const int64_t jobs = (a.total + window - 1) / window * a.c.heads * 2;
+  const unsigned grid = (unsigned)((jobs + kWarps - 1) / kWarps);
+  if (bf16) append_kernel<D, E4M3, true><<<grid, kWarps * 32, 0, s>>>(a);
+  else append_kernel<D, E4M3, false><<<grid, kWarps * 32, 0, s>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_append(const AppendArgs& a, bool e4m3, bool bf16, cudaStream_t s) {
+  switch (a.c.dim) {
+    case 64: return e4m3 ? launch_append_d<64, true>(a, bf16, s) : launch_append_d<64, false>(a, bf16, s);
+    case 128: return e4m3 ? launch_append_d<128, true>(a, bf16, s) : launch_append_d<128, false>(a, bf16, s);
+    default: return e4m3 ? launch_append_d<256, true>(a, bf16, s) : launch_append_d<256, false>(a, bf16, s);
+  }
+}
+
+}  // namespace kv8
+}  // namespace fa

@@ -302,6 +302,127 @@ class PagedKVCache(BlockManager):
                                           self.max_blocks_per_seq, cu_seqlens=cu_seqlens, return_k=True)
 
 
+class PagedKVCache8(BlockManager):
+    """K and V pools in 8 bits, `[num_blocks, H_KV, 16, D]` per layer with a scale for each block, head and kind, and eviction by
+    the weights that attention gave the tokens.
+
+    `codes` is torch.int8 or torch.float8_e4m3fn.  With `eviction` every layer keeps the sums of weights of each request's
+    tokens, [max_batch, H_KV, tokens] in fp32, which `attend` adds to and `evict` goes by.  A request that was cut has
+    `get_cache_len` tokens in the cache and `position` tokens behind it: rotary angles go by the latter."""
+
+    def __init__(self, num_blocks: int, num_layers: int, num_kv_heads: int, head_dim: int, max_batch: int, max_blocks_per_seq: int,
+                 device="cuda", codes=torch.int8, enable_prefix_cache: bool = True, eviction: bool = True):
+        if num_layers <= 0:
+            raise ValueError("num_layers must be positive")
+        if codes not in (torch.int8, torch.float8_e4m3fn):
+            raise ValueError("codes must be torch.int8 or torch.float8_e4m3fn")
+        super().__init__(num_blocks, max_batch, max_blocks_per_seq, device, enable_prefix_cache)
+        self.num_layers = num_layers
+        self.num_kv_heads, self.head_dim = num_kv_heads, head_dim
+        shape = (num_blocks, num_kv_heads, BLOCK_SIZE, head_dim)
+        pools = lambda: [torch.zeros(shape, dtype=torch.int8, device=self.device).view(codes) for _ in range(num_layers)]
+        self.k_pools, self.v_pools = pools(), pools()
+        self.scales = [torch.zeros((num_blocks, num_kv_heads, 2), device=self.device) for _ in range(num_layers)]
+        self.masses = [torch.zeros((max_batch, num_kv_heads, max_blocks_per_seq * BLOCK_SIZE), device=self.device)
+                       for _ in range(num_layers)] if eviction else None
+        self._positions: Dict[str, int] = {}                     # request -> tokens it has had
+
+    # ---- bookkeeping ----------------------------------------------------------------
+    def allocate(self, request_id: str, num_tokens: int = 0, token_ids: Optional[Sequence[int]] = None) -> int:
+        row = super().allocate(request_id, num_tokens, token_ids)
+        self._positions[request_id] = self._tokens[request_id]
+        for m in self.masses or ():
+            m[row].zero_()
+        return row
+
+    def commit(self, request_id: str, num_new_tokens: int) -> None:
+        super().commit(request_id, num_new_tokens)
+        self._positions[request_id] += num_new_tokens
+
+    def release(self, request_id: str) -> None:
+        super().release(request_id)
+        self._positions.pop(request_id, None)
+
+    def position(self, request_id: str) -> int:
+        """Tokens the request has had, evicted ones among them: the position of its next token."""
+        return self._positions[request_id]
+
+    def cache_prefix(self, token_ids: Sequence[int], request_id: str) -> int:
+        if self._positions.get(request_id) != self._tokens.get(request_id):
+            return 0                                              # what is left is no prefix
+        return super().cache_prefix(token_ids, request_id)
+
+    # ---- data path ------------------------------------------------------------------
+    def _append(self, layer, request_ids, q, k, v, cos, sin, cu_seqlens):
+        from . import kv8_ops, ops
+        table, lens = self.batch_view(request_ids)
+        rotate = ops.rope_append_paged_bf16 if q.dtype == torch.bfloat16 else ops.rope_append_paged_fp16
+        q, k = rotate(q, k, v, cos, sin, None, None, None, lens if cu_seqlens is None else None, 0, cu_seqlens=cu_seqlens, return_k=True)
+        kv8_ops.append_paged_kv8(k, v, self.k_pools[layer], self.v_pools[layer], self.scales[layer], table, lens, self.max_blocks_per_seq,
+                                 cu_seqlens=cu_seqlens)
+        return q, k
+
+    def append_decode(self, layer: int, request_ids: Sequence[str], q, k, v, cos, sin):
+        """One decode step for one layer: rotate q / k and store k, v of each request's new token at its next slot; returns the
+        rotated q.  Call `reserve` (once per step) before, `commit` (once per step) after."""
+        return self._append(layer, request_ids, q, k, v, cos, sin, None)[0]
+
+    def append_prefill(self, layer: int, request_ids: Sequence[str], q, k, v, cos, sin, cu_seqlens):
+        """Packed prompts for one layer: rotate q / k, store k / v from each request's current length on; returns
+        (q_rot, k_rot) for the prefill attention."""
+        return self._append(layer, request_ids, q, k, v, cos, sin, cu_seqlens)
+
+    def attend(self, layer: int, request_ids: Sequence[str], q, softcap: float = 0.0, track: bool = True):
+        """Attention of q [B, H_Q, T, D], each request's newest T tokens (appended, not committed yet); with `track` (and `eviction`)
+        their weights are added to the tokens' sums."""
+        from . import kv8_ops
+        table, lens = self.batch_view(request_ids, extra_tokens=q.size(2))
+        mass = self.masses[layer] if track and self.masses is not None else None
+        rows = None
+        if mass is not None:
+            rows = torch.tensor([self._row[r] for r in request_ids], dtype=torch.int32).to(self.device)
+        return kv8_ops.forward_paged_decode_gqa_kv8(q, self.k_pools[layer], self.v_pools[layer], self.scales[layer], table, lens,
+                                                    self.max_blocks_per_seq, softcap=softcap, mass=mass, mass_index=rows)
+
+    def evict(self, request_ids: Sequence[str], budget: int, sink: int = 4, recent: int = 64) -> int:
+        """Cut every request of more than `budget` committed tokens to `budget`, layer by layer and head by head; returns the blocks
+        that came free.  The tokens move to new blocks, so blocks that other requests or a prefix share stay as they are; there must
+        be enough free ones for the requests that are cut."""
+        from . import kv8_ops
+        if self.masses is None:
+            raise RuntimeError("this cache keeps no sums of weights (eviction=False)")
+        if budget <= 0 or sink < 0 or recent < 0 or sink + recent > budget:
+            raise ValueError("budget must be positive and hold sink and recent")
+        if len(set(request_ids)) != len(request_ids):
+            raise ValueError("a request is named twice")
+        ids = [r for r in request_ids if self._tokens[r] > budget]
+        if not ids:
+            return 0
+        free = len(self._free)
+        n = (budget + BLOCK_SIZE - 1) // BLOCK_SIZE
+        blocks = self._take_blocks(n * len(ids))
+        new = [blocks[i * n: (i + 1) * n] for i in range(len(ids))]
+        table, lens = self.batch_view(ids)
+        new_table = torch.tensor(new, dtype=torch.int32).to(self.device)
+        rows = torch.tensor([self._row[r] for r in ids], dtype=torch.int32).to(self.device)
+        at = rows.long()
+        for layer in range(self.num_layers):
+            mass = self.masses[layer]
+            _, _, kept = kv8_ops.evict_paged_kv8(mass, self.k_pools[layer], self.v_pools[layer], self.scales[layer], table, lens,
+                                                 self.max_blocks_per_seq, new_table, budget, sink, recent, mass_index=rows)
+            mass[at] = torch.nn.functional.pad(kept, (0, mass.size(2) - budget))
+        for r, own in zip(ids, new):
+            row, old = self._row[r], self._tables[r]
+            self._tables[r] = list(own)
+            self._tokens[r] = budget
+            self.block_table[row, : len(old)] = -1
+            self.block_table[row, :n] = torch.tensor(own, dtype=torch.int32)
+            for b in reversed(old):
+                if b >= 0:
+                    self._drop_ref(b)
+        return len(self._free) - free
+
+
 class HybridCache(BlockManager):
     """What the layer runs of a hybrid decoder keep per request, behind one block table.
 

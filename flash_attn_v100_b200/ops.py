@@ -16,6 +16,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import functools
+import sys
 import threading
 from typing import Dict, Tuple
 
@@ -213,7 +214,11 @@ def _workspace(device, stream_int, B, H_Q, H_KV, D):
 
 def check_async_errors(device=None) -> None:
     """Synchronise and raise RuntimeError if a decode kernel on `device` recorded a
-    bounded-wait timeout or an out-of-pool page id since its workspace was created."""
+    bounded-wait timeout or an out-of-pool page id since its workspace was created, or an operator
+    on an 8-bit cache a page outside it."""
+    kv8 = sys.modules.get(f"{__package__}.kv8_ops")
+    if kv8 is not None:
+        kv8.check_errors(device)
     lib = _lib.load()
     for (dev, stream_int), ws in list(_workspaces.items()):
         if device is not None and torch.device(device).index not in (None, dev):

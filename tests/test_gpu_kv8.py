@@ -1,0 +1,552 @@
+"""GPU: the operators on the paged 8-bit cache against the CPU oracle.  Codes, scales, kept tokens and their sums are compared bit for bit;
+attention goes by the bound that tests/kv8_cases.py derives."""
+import math
+
+import pytest
+import torch
+
+import kv8_cases as kc
+from oracle import kv8_oracle as orc
+
+pytestmark = pytest.mark.gpu
+CODES = kc.CODES
+
+
+@pytest.fixture(scope="module")
+def fa():
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    import flash_attn_v100_b200
+    return flash_attn_v100_b200
+
+
+@pytest.fixture(autouse=True)
+def no_errors(fa):
+    yield
+    torch.cuda.synchronize()
+    fa.check_async_errors()
+
+
+def _same(got, want):
+    got = got.cpu()
+    assert got.dtype == want.dtype and got.shape == want.shape
+    assert torch.equal(kc.bits(got), kc.bits(want)), (kc.bits(got) != kc.bits(want)).sum().item()
+
+
+def _ints(v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+# ---- append --------------------------------------------------------------------------------------------------------
+def _append_both(fa, k, v, kc0, vc0, sc0, table, positions, cu, mutate=lambda t: t):
+    dev = [t.cuda() for t in (kc0, vc0, sc0)]
+    fa.append_paged_kv8(mutate(k.cuda()), mutate(v.cuda()), *dev, table.cuda(), None if positions is None else positions.cuda(), table.size(1),
+                        cu_seqlens=None if cu is None else cu.cuda())
+    ref = [t.clone() for t in (kc0, vc0, sc0)]
+    flat = lambda t: t.reshape(-1, t.size(1), t.size(-1)) if cu is None else t
+    orc.append(flat(k), flat(v), *ref, table, positions, cu)
+    for got, want in zip(dev, ref):
+        _same(got, want)
+    return dev, ref
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,H", [(64, 2), (128, 3), (256, 1)])
+def test_append_packed_prompts(fa, codes, dtype, D, H):
+    lens, starts = [1, 0, 15, 16, 17, 40, 0, 3, 33], [0, 5, 1, 0, 16, 30, 2, 14, 15]
+    total = [a + n for a, n in zip(starts, lens)]
+    table, rest = kc.tables(total, 40, 1)
+    g = torch.Generator().manual_seed(D + H)
+    k, v = ((torch.randn(sum(lens), H, D, generator=g) * s).to(dtype) for s in (3.0, 0.02))
+    cu = _ints([0] + torch.tensor(lens).cumsum(0).tolist())
+    _append_both(fa, k, v, *kc.cache(40, H, D, codes, 2), table, _ints(starts), cu)
+    _append_both(fa, k, v, *kc.cache(40, H, D, codes, 3), table, None, cu)
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_append_steps_grow_the_scale(fa, codes, D):
+    """Forty steps of three sequences: a page's scale grows as larger rows come, its codes are rounded again, a new page begins anew."""
+    H, B = 2, 3
+    table, _ = kc.tables([50, 57, 64], 12, 4)
+    state = kc.cache(12, H, D, codes, 5)
+    dev, ref = [t.cuda() for t in state], [t.clone() for t in state]
+    g = torch.Generator().manual_seed(6)
+    for step in range(40):
+        k, v = (torch.randn(B, H, 1, D, generator=g).mul(1 + 0.2 * step).half() for _ in range(2))
+        pos = _ints([step, step + 7, step + 15])
+        fa.append_paged_kv8(k.cuda(), v.cuda(), *dev, table.cuda(), pos.cuda(), table.size(1))
+        orc.append(k[:, :, 0], v[:, :, 0], *ref, table, pos)
+    for got, want in zip(dev, ref):
+        _same(got, want)
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_append_values_at_the_edges(fa, codes, dtype):
+    """Zeros, the least and the largest values, infinities and NaN; also into a page that has rows."""
+    D, H = 64, 1
+    rows = torch.randn(12, H, D, generator=torch.Generator().manual_seed(7)).to(dtype)
+    top = torch.finfo(dtype).max
+    rows[0] = 0
+    rows[1] = torch.finfo(dtype).smallest_normal
+    rows[2] = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps           # least subnormal
+    rows[3, 0, 3] = top
+    rows[4, 0, 5] = math.inf
+    rows[5, 0, 7] = -math.inf
+    rows[6, 0, 9] = math.nan
+    rows[7] = -0.0
+    rows[8] = torch.arange(D).to(dtype) / D - 0.5
+    for start in (0, 3):
+        n = rows.size(0)
+        table, _ = kc.tables([start + 1] * n, n, 8)
+        cu = _ints(range(n + 1))
+        _append_both(fa, rows, rows.flip(0), *kc.cache(n, H, D, codes, 9), table, _ints([start] * n), cu)
+
+
+def test_append_takes_slices_of_a_fused_projection(fa):
+    H, D, n = 2, 128, 37
+    g = torch.Generator().manual_seed(10)
+    fused = torch.randn(n, 4 * H * D, generator=g).half().cuda()
+    k, v = fused[:, H * D: 2 * H * D].view(n, H, D), fused[:, 3 * H * D:].view(n, H, D)
+    assert not k.is_contiguous()
+    table, _ = kc.tables([n], 4, 11)
+    state = kc.cache(4, H, D, torch.int8, 12)
+    dev, ref = [t.cuda() for t in state], [t.clone() for t in state]
+    fa.append_paged_kv8(k, v, *dev, table.cuda(), None, table.size(1), cu_seqlens=_ints([0, n]).cuda())
+    orc.append(k.cpu(), v.cpu(), *ref, table, None, _ints([0, n]))
+    for got, want in zip(dev, ref):
+        _same(got, want)
+    # a decode step on one row of a fused projection per sequence
+    kd, vd = (t[:3].unsqueeze(2) for t in (k, v))
+    table3, _ = kc.tables([16, 20, 1], 4, 13)
+    fa.append_paged_kv8(kd, vd, *dev, table3.cuda(), _ints([15, 19, 0]).cuda(), table3.size(1))
+    orc.append(kd[:, :, 0].cpu(), vd[:, :, 0].cpu(), *ref, table3, _ints([15, 19, 0]))
+    for got, want in zip(dev, ref):
+        _same(got, want)
+
+
+def test_append_leaves_bad_pages_alone(fa):
+    H, D = 2, 64
+    state = kc.cache(4, H, D, torch.int8, 14)
+    table = _ints([[0, 7], [-1, 1], [2, 3]])
+    k = torch.randn(3 * 20, H, D, generator=torch.Generator().manual_seed(15)).half()
+    dev, ref = [t.cuda() for t in state], [t.clone() for t in state]
+    # pages 7 and -1 are outside the cache, and tokens 32 to 39 of the last sequence have no entry of the table
+    fa.append_paged_kv8(k.cuda(), k.cuda(), *dev, table.cuda(), _ints([0, 0, 20]).cuda(), 2, cu_seqlens=_ints([0, 20, 40, 60]).cuda())
+    with pytest.raises(RuntimeError, match="outside the cache"):
+        fa.check_async_errors()
+    fa.check_async_errors()
+    for rows, page, slot in ((k[:16], 0, 0), (k[36:40], 1, 0), (k[40:52], 3, 4)):
+        orc.append(rows, rows, *ref, _ints([[page]]), _ints([slot]), _ints([0, rows.size(0)]))
+    for got, want in zip(dev, ref):
+        _same(got, want)
+
+
+# ---- decode --------------------------------------------------------------------------------------------------------
+def _decode_case(fa, codes, dtype, H, G, D, T, lens, seed, softcap=0.0, mass=False, q_scale=1.0):
+    pages = sum((max(0, n) + 15) // 16 for n in lens) + 3
+    table, rest = kc.tables(lens, pages, seed)
+    k8, v8, scale = kc.cache(pages, H, D, codes, seed + 1)
+    for p in rest:                                    # pages of nobody: whoever reads them shows
+        scale[p] = math.nan
+    g = torch.Generator().manual_seed(seed + 2)
+    q = (torch.randn(len(lens), H * G, T, D, generator=g) * q_scale).to(dtype)
+    sums = torch.rand(len(lens) + 2, H, table.size(1) * 16 + 5, generator=g) if mass else None
+    index = torch.randperm(len(lens) + 2, generator=g)[: len(lens)].int() if mass else None
+    dev = sums.cuda() if mass else None
+    out = fa.forward_paged_decode_gqa_kv8(q.cuda(), k8.cuda(), v8.cuda(), scale.cuda(), table.cuda(), _ints(lens).cuda(), table.size(1), softcap=softcap,
+                                          mass=dev, mass_index=index.cuda() if mass else None)
+    assert out.shape == q.shape and out.dtype == dtype
+    sums64 = sums.double() if mass else None
+    used = scale.clone()
+    for p in rest:
+        used[p] = 0
+    ref, size = orc.decode(q, k8, v8, used, table, lens, softcap, sums64, index)
+    bound, delta = kc.decode_bound(q, k8, used, ref, size, dtype, softcap)
+    off = (out.cpu().double() - ref).abs()
+    assert bool((off <= bound).all()), (off / bound).max().item()
+    if mass:
+        got = dev.cpu().double()
+        added = sums64 - sums.double()
+        limit = added * (2 * delta + 2.0 ** -18) + sums64 * 2.0 ** -23
+        assert bool(((got - sums64).abs() <= limit).all())
+        assert torch.equal(dev.cpu()[added == 0], sums[added == 0])
+    return out
+
+
+LENS = [0, 1, 15, 16, 17, 33, 100, 257]
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("G", [1, 4, 8, 12])
+def test_decode_shapes(fa, codes, dtype, D, G):
+    _decode_case(fa, codes, dtype, 2, G, D, 1, LENS, 20 + G)
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("H,G,T", [(1, 1, 1), (3, 5, 1), (2, 20, 1), (1, 4, 4), (2, 5, 3), (2, 1, 40), (1, 3, 17)])
+def test_decode_groups_and_guessed_tokens(fa, codes, H, G, T):
+    _decode_case(fa, codes, torch.bfloat16, H, G, 128, T, LENS + [40], 30 + G + T, mass=True)
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("D,G", [(64, 4), (128, 9), (256, 4)])
+@pytest.mark.parametrize("softcap", [0.0, 5.0, 50.0])
+def test_decode_capped_and_summed(fa, codes, D, G, softcap):
+    _decode_case(fa, codes, torch.float16, 2, G, D, 2, LENS, 40 + G, softcap=softcap, mass=True, q_scale=2.0)
+
+
+@pytest.mark.parametrize("lens", [[5000], [4097, 3], [31, 3000, 1, 16], [700] * 5, [64] * 160], ids=str)
+@pytest.mark.parametrize("codes", CODES)
+def test_decode_cut_into_parts(fa, codes, lens):
+    """Few long sequences (parts for CTAs of their own), and enough sequences for an even cut through all of them."""
+    _decode_case(fa, codes, torch.float16, 2, 4, 128, 1, lens, 50 + len(lens), mass=len(lens) < 100)
+
+
+def test_decode_even_cut_of_unequal_sequences(fa):
+    lens = [(37 * i) % 500 for i in range(200)]
+    _decode_case(fa, torch.int8, torch.float16, 2, 2, 64, 1, lens, 60, mass=True)
+
+
+def test_decode_of_more_sequences_than_a_launch_takes(fa):
+    lens = [i % 3 for i in range(4100)]
+    _decode_case(fa, torch.int8, torch.float16, 1, 1, 64, 1, lens, 61)
+
+
+@pytest.mark.parametrize("codes", CODES)
+def test_decode_scales_of_all_sizes(fa, codes):
+    """Pages whose scales differ by 2^40 and pages of zeros under a scale of 0: the large ones decide the result, all of them the weights."""
+    H, D, lens = 1, 64, [100, 64]
+    table, _ = kc.tables(lens, 12, 62)
+    k8, v8, scale = kc.cache(12, H, D, codes, 63)
+    g = torch.Generator().manual_seed(64)
+    scale[..., 1] = torch.exp2(torch.randint(-20, 21, (12, H), generator=g).float())
+    zero = int(table[0, 2])
+    scale[zero] = 0.0
+    q = torch.randn(2, 4, 1, D, generator=g).bfloat16()
+    out = fa.forward_paged_decode_gqa_kv8(q.cuda(), k8.cuda(), v8.cuda(), scale.cuda(), table.cuda(), _ints(lens).cuda(), table.size(1))
+    ref, size = orc.decode(q, k8, v8, scale, table, lens)
+    bound, _ = kc.decode_bound(q, k8, scale, ref, size, torch.bfloat16, 0.0)
+    assert bool(((out.cpu().double() - ref).abs() <= bound).all())
+
+
+def test_decode_spoiled_pages_spoil_what_sees_them(fa):
+    """An infinite scale (a page that was given NaN) makes the rows that see it NaN and no others; codes behind a sequence's end are not seen."""
+    H, D, lens = 1, 64, [40, 40]
+    table, _ = kc.tables(lens, 6, 65)
+    k8, v8, scale = kc.cache(6, H, D, torch.float8_e4m3fn, 66)
+    kc.bits(k8)[int(table[1, 2]), :, 8:] = 0x7F                                  # NaN behind token 39
+    kc.bits(v8)[int(table[1, 2]), :, 8:] = 0x7F
+    q = torch.randn(2, 4, 1, D, generator=torch.Generator().manual_seed(67)).half()
+    args = lambda s: (q.cuda(), k8.cuda(), v8.cuda(), s.cuda(), table.cuda(), _ints(lens).cuda(), table.size(1))
+    fine = fa.forward_paged_decode_gqa_kv8(*args(scale))
+    assert bool(fine.isfinite().all())
+    for kind in (0, 1):
+        bad = scale.clone()
+        bad[int(table[0, 1]), 0, kind] = math.inf
+        kc.bits(k8 if kind == 0 else v8)[int(table[0, 1])] = 0
+        out = fa.forward_paged_decode_gqa_kv8(*args(bad))
+        assert bool(out[0].isnan().all()) and torch.equal(out[1], fine[1])
+
+
+def test_decode_reports_bad_pages(fa):
+    H, D, lens = 1, 64, [40, 20]
+    table, _ = kc.tables(lens, 6, 68)
+    table[0, 1] = 6
+    q = torch.zeros(2, 1, 1, D).half().cuda()
+    k8, v8, scale = (t.cuda() for t in kc.cache(6, H, D, torch.int8, 69))
+    out = fa.forward_paged_decode_gqa_kv8(q, k8, v8, scale, table.cuda(), _ints(lens).cuda(), table.size(1))
+    assert bool(out[1].isfinite().all())
+    with pytest.raises(RuntimeError, match="outside the cache"):
+        fa.check_async_errors()
+
+
+def test_decode_lengths_beyond_the_table_are_cut(fa):
+    H, D = 1, 64
+    table, _ = kc.tables([32], 4, 70)
+    k8, v8, scale = (t.cuda() for t in kc.cache(4, H, D, torch.int8, 71))
+    q = torch.randn(1, 2, 1, D, generator=torch.Generator().manual_seed(72)).half().cuda()
+    run = lambda n: fa.forward_paged_decode_gqa_kv8(q, k8, v8, scale, table.cuda(), _ints([n]).cuda(), 2)
+    assert torch.equal(run(1000), run(32)) and bool((run(-3) == 0).all())
+
+
+def test_caches_of_more_than_32_bits(fa):
+    """Pages whose codes lie beyond 2^32 bytes."""
+    H, D, lens = 8, 256, [50]
+    pages = (1 << 32) // (H * 16 * D) + 40
+    table = _ints([[pages - 1, pages - 30, pages - 2, pages - 7]])
+    k8, v8 = (torch.empty((pages, H, 16, D), dtype=torch.int8, device="cuda") for _ in range(2))
+    scale = torch.empty((pages, H, 2), device="cuda")
+    g = torch.Generator().manual_seed(73)
+    k, v = (torch.randn(50, H, D, generator=g).half() for _ in range(2))
+    fa.append_paged_kv8(k.cuda(), v.cuda(), k8, v8, scale, table.cuda(), None, 4, cu_seqlens=_ints([0, 50]).cuda())
+    q = torch.randn(1, 16, 1, D, generator=g).half()
+    out = fa.forward_paged_decode_gqa_kv8(q.cuda(), k8, v8, scale, table.cuda(), _ints(lens).cuda(), 4)
+    mass = torch.rand(1, H, 64, generator=g)
+    new = _ints([[pages - 12, pages - 3]])
+    kept, _, _ = fa.evict_paged_kv8(mass.cuda(), k8, v8, scale, table.cuda(), _ints(lens).cuda(), 4, new.cuda(), 20, 2, 3)
+    small = [torch.zeros((6, H, 16, D), dtype=torch.int8) for _ in range(2)] + [torch.zeros(6, H, 2)]
+    near = _ints([[0, 1, 2, 3]])
+    orc.append(k, v, *small, near, None, _ints([0, 50]))
+    ref, size = orc.decode(q, *small, near, lens)
+    bound, _ = kc.decode_bound(q, small[0], small[2], ref, size, torch.float16, 0.0)
+    assert bool(((out.cpu().double() - ref).abs() <= bound).all())
+    want, _, _ = orc.evict(mass, *small, near, lens, _ints([[4, 5]]), 20, 2, 3)
+    assert torch.equal(kept.cpu(), want)
+    for i, p in enumerate(new[0].tolist()):
+        n = 16 if i == 0 else 4
+        assert torch.equal(k8[p, :, :n].cpu(), small[0][4 + i, :, :n]) and torch.equal(v8[p, :, :n].cpu(), small[1][4 + i, :, :n])
+        assert torch.equal(scale[p].cpu(), small[2][4 + i])
+
+
+# ---- eviction -------------------------------------------------------------------------------------------------------
+def _evict_case(fa, codes, H, D, lens, budget, sink, recent, seed, mass=None, index=None):
+    new_pages = (budget + 15) // 16
+    pages = sum((max(0, n) + 15) // 16 for n in lens) + new_pages * len(lens) + 2
+    table, rest = kc.tables(lens, pages, seed)
+    new = _ints([rest[b * new_pages: (b + 1) * new_pages] for b in range(len(lens))])
+    state = kc.cache(pages, H, D, codes, seed + 1)
+    if mass is None:
+        g = torch.Generator().manual_seed(seed + 2)
+        mass = torch.randn(len(lens), H, table.size(1) * 16, generator=g).exp()
+        mass *= torch.rand(mass.shape, generator=g) > 0.2
+    dev, ref = [t.cuda() for t in state], [t.clone() for t in state]
+    got = fa.evict_paged_kv8(mass.cuda(), *dev, table.cuda(), _ints(lens).cuda(), table.size(1), new.cuda(), budget, sink, recent,
+                             mass_index=None if index is None else index.cuda())
+    want = orc.evict(mass, *ref, table, lens, new, budget, sink, recent, index)
+    for a, b in zip(got[:2], want[:2]):
+        assert torch.equal(a.cpu(), b)
+    assert torch.equal(got[2].cpu().nan_to_num(-1.0), want[2].nan_to_num(-1.0))
+    for a, b in zip(dev, ref):
+        _same(a, b)
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("budget,sink,recent", [(1, 0, 0), (16, 4, 3), (50, 0, 50), (33, 33, 0), (100, 10, 17)])
+def test_evict_sizes(fa, codes, D, budget, sink, recent):
+    _evict_case(fa, codes, 2, D, LENS + [101, 99], budget, sink, recent, 80 + budget)
+
+
+def test_evict_equal_sums_keep_the_first(fa):
+    lens, H = [300, 2500], 2
+    mass = torch.zeros(2, H, 2512)
+    mass[:, 1] = torch.randint(0, 3, (2, 2512), generator=torch.Generator().manual_seed(81)).float()
+    mass[0, 0, ::2] = -0.0
+    _evict_case(fa, torch.int8, H, 64, lens, 130, 3, 20, 82, mass)
+
+
+def test_evict_odd_sums(fa):
+    """Negative sums, infinities and NaN have their places in the order too."""
+    g = torch.Generator().manual_seed(83)
+    mass = torch.randn(3, 1, 416, generator=g)
+    mass[0, 0, ::7] = math.nan
+    mass[1, 0, ::5] = math.inf
+    mass[2, 0, ::3] = -math.inf
+    mass[2, 0, 1::3] = -1e-42
+    _evict_case(fa, torch.float8_e4m3fn, 1, 64, [400, 401, 390], 120, 2, 9, 84, mass)
+
+
+@pytest.mark.parametrize("lens,budget", [([20000], 3001), ([9000, 8191, 40], 512), ([70000], 5)])
+def test_evict_long_sequences(fa, lens, budget):
+    """Rows that a cluster of CTAs shares."""
+    _evict_case(fa, torch.int8, 2, 64, lens, budget, min(4, budget), 0, 85)
+
+
+def test_evict_rows_of_sums_by_index(fa):
+    g = torch.Generator().manual_seed(86)
+    _evict_case(fa, torch.int8, 2, 64, [100, 60, 80], 40, 1, 5, 87, torch.rand(7, 2, 128, generator=g), _ints([5, 0, 3]))
+
+
+def test_evict_reports_rows_and_pages_outside(fa):
+    H, D = 1, 64
+    state = [t.cuda() for t in kc.cache(8, H, D, torch.int8, 88)]
+    before = [t.clone() for t in state]
+    mass = torch.rand(2, H, 32, generator=torch.Generator().manual_seed(89)).cuda()
+    table, lens = _ints([[0, 1], [2, 3]]).cuda(), _ints([32, 32]).cuda()
+    _, n, _ = fa.evict_paged_kv8(mass, *state, table, lens, 2, _ints([[4], [9]]).cuda(), 16, mass_index=_ints([2, 0]).cuda())
+    assert n.tolist() == [0, 16]
+    with pytest.raises(RuntimeError, match="outside the cache"):
+        fa.check_async_errors()
+    for a, b in zip(state, before):
+        _same(a, b.cpu())
+
+
+# ---- together ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("codes", CODES)
+def test_prompts_steps_and_eviction_in_a_row(fa, codes):
+    """A short service: prompts in, steps with sums, a cut, more steps on what is left, each held against the oracle on the oracle's own cache."""
+    H, G, D, B, budget = 2, 4, 64, 3, 40
+    lens = [70, 33, 50]
+    pages = 40
+    table, rest = kc.tables([96] * B, pages, 90, width=6)
+    new = _ints([rest[i * 6: i * 6 + 6] for i in range(B)])
+    state = kc.cache(pages, H, D, codes, 91)
+    dev, ref = [t.cuda() for t in state], [t.clone() for t in state]
+    g = torch.Generator().manual_seed(92)
+    rnd = lambda *s: torch.randn(*s, generator=g).bfloat16()
+    k, v = rnd(sum(lens), H, D), rnd(sum(lens), H, D)
+    cu = _ints([0, 70, 103, 153])
+    fa.append_paged_kv8(k.cuda(), v.cuda(), *dev, table.cuda(), None, 6, cu_seqlens=cu.cuda())
+    orc.append(k, v, *ref, table, None, cu)
+    mass, mass64 = torch.zeros(B, H, 96).cuda(), torch.zeros(B, H, 96, dtype=torch.float64)
+
+    def steps(n, table, lens):
+        for _ in range(n):
+            k, v, q = rnd(B, H, 1, D), rnd(B, H, 1, D), rnd(B, H * G, 1, D)
+            fa.append_paged_kv8(k.cuda(), v.cuda(), *dev, table.cuda(), _ints(lens).cuda(), 6)
+            orc.append(k[:, :, 0], v[:, :, 0], *ref, table, _ints(lens))
+            lens = [n + 1 for n in lens]
+            out = fa.forward_paged_decode_gqa_kv8(q.cuda(), *dev, table.cuda(), _ints(lens).cuda(), 6, mass=mass)
+            want, size = orc.decode(q, *ref, table, lens, mass=mass64)
+            bound, _ = kc.decode_bound(q, ref[0], ref[2], want, size, torch.bfloat16, 0.0)
+            assert bool(((out.cpu().double() - want).abs() <= bound).all())
+        for got, want in zip(dev, ref):
+            _same(got, want)
+        return lens
+
+    lens = steps(5, table, lens)
+    sums = mass.cpu()
+    assert bool(((sums.double() - mass64).abs() <= 1e-2 * mass64 + 1e-9).all())
+    kept, new_lens, new_mass = fa.evict_paged_kv8(mass, *dev, table.cuda(), _ints(lens).cuda(), 6, new.cuda(), budget, 2, 8)
+    want = orc.evict(sums, *ref, table, lens, new, budget, 2, 8)
+    for a, b in zip((kept, new_lens, new_mass), want):
+        assert torch.equal(a.cpu(), b)
+    mass.zero_(); mass64.zero_()
+    mass[:, :, :budget] = new_mass
+    mass64[:, :, :budget] = new_mass.cpu().double()
+    lens = steps(20, new, new_lens.tolist())
+    assert lens == [60, 58, 60]
+
+
+def test_calls_on_another_stream_and_in_a_graph(fa):
+    """A step captured once (append, attention with sums) and replayed with other inputs does what eager calls do, also beside a second graph on another stream."""
+    H, G, D, B = 2, 4, 128, 4
+    lens = [900, 33, 16, 250]
+    pages = 100
+    table, _ = kc.tables([n + 32 for n in lens], pages, 93)
+    g = torch.Generator().manual_seed(94)
+    rows = lambda: [torch.randn(B, n, 1, D, generator=g).half().cuda() for n in (H, H, H * G)]
+    sets = []
+    for i in range(2):
+        dev = [t.cuda() for t in kc.cache(pages, H, D, torch.int8, 95 + i)]
+        sets.append(dict(dev=dev, copy=[t.clone() for t in dev], k=rows(), lens=_ints(lens).cuda(), pos=(_ints(lens) - 1).cuda(),
+                         mass=torch.zeros(B, H, table.size(1) * 16).cuda(), graph=torch.cuda.CUDAGraph(), stream=torch.cuda.Stream()))
+    bt = table.cuda()
+
+    def step(s, dev, mass):
+        fa.append_paged_kv8(s["k"][0], s["k"][1], *dev, bt, s["pos"], bt.size(1))
+        return fa.forward_paged_decode_gqa_kv8(s["k"][2], *dev, bt, s["lens"], bt.size(1), mass=mass)
+
+    for s in sets:
+        with torch.cuda.stream(s["stream"]):                      # first calls outside the capture
+            step(s, [t.clone() for t in s["dev"]], s["mass"].clone())
+            s["stream"].synchronize()
+            with torch.cuda.graph(s["graph"], stream=s["stream"]):
+                s["out"] = step(s, s["dev"], s["mass"])
+    torch.cuda.synchronize()
+    for round_ in range(3):
+        fresh = [rows() for _ in sets]
+        for s, f in zip(sets, fresh):
+            for a, b in zip(s["k"], f):
+                a.copy_(b)
+        torch.cuda.synchronize()
+        for s in sets:
+            with torch.cuda.stream(s["stream"]):
+                s["graph"].replay()
+        torch.cuda.synchronize()
+        for s in sets:
+            mass = s.setdefault("mass2", torch.zeros_like(s["mass"]))
+            out = step(s, s["copy"], mass)
+            torch.cuda.synchronize()
+            assert torch.equal(out, s["out"]) and torch.equal(mass, s["mass"])
+            for a, b in zip(s["dev"], s["copy"]):
+                assert torch.equal(kc.bits(a), kc.bits(b))
+        for s in sets:
+            s["lens"].add_(1); s["pos"].add_(1)
+
+
+def test_results_do_not_change_from_call_to_call(fa):
+    lens = [3000, 17, 900]
+    table, _ = kc.tables(lens, 260, 96)
+    k8, v8, scale = (t.cuda() for t in kc.cache(260, 4, 128, torch.int8, 97))
+    q = torch.randn(3, 16, 1, 128, generator=torch.Generator().manual_seed(98)).half().cuda()
+    outs = []
+    for _ in range(20):
+        mass = torch.zeros(3, 4, table.size(1) * 16).cuda()
+        outs.append((fa.forward_paged_decode_gqa_kv8(q, k8, v8, scale, table.cuda(), _ints(lens).cuda(), table.size(1), mass=mass), mass))
+    assert all(torch.equal(a, outs[0][0]) and torch.equal(b, outs[0][1]) for a, b in outs)
+
+
+def test_empty_calls(fa):
+    k8, v8, scale = (t.cuda() for t in kc.cache(2, 1, 64, torch.int8, 99))
+    table, none = torch.zeros((0, 1), dtype=torch.int32).cuda(), torch.zeros(0, dtype=torch.int32).cuda()
+    assert fa.forward_paged_decode_gqa_kv8(torch.zeros(0, 1, 1, 64).half().cuda(), k8, v8, scale, table, none, 1).shape == (0, 1, 1, 64)
+    fa.append_paged_kv8(*[torch.zeros(0, 1, 1, 64).half().cuda()] * 2, k8, v8, scale, table, none, 1)
+    fa.append_paged_kv8(*[torch.zeros(0, 1, 64).half().cuda()] * 2, k8, v8, scale, torch.zeros((1, 1), dtype=torch.int32).cuda(), None, 1,
+                        cu_seqlens=_ints([0, 0]).cuda())
+    kept, n, m = fa.evict_paged_kv8(torch.zeros(1, 1, 16).cuda(), k8, v8, scale, table, none, 1, table, 16)
+    assert kept.shape == (0, 1, 16) and n.numel() == 0 and m.shape == (0, 1, 16)
+
+
+# ---- the cache class -------------------------------------------------------------------------------------------------
+def test_cache_class_serves_and_evicts(fa):
+    """Prompts, steps, a cut that leaves a shared prefix in place, and steps after it, against the operators' oracle."""
+    H, G, D = 2, 2, 64
+    c = fa.PagedKVCache8(64, 2, H, D, max_batch=4, max_blocks_per_seq=16, codes=torch.int8)
+    g = torch.Generator().manual_seed(100)
+    rnd = lambda *s: torch.randn(*s, generator=g).half().cuda()
+    prompt = list(range(80))
+    c.allocate("a", 80, prompt)
+    cu = _ints([0, 80]).cuda()
+    turn = lambda n: (torch.ones(n, D).cuda(), torch.zeros(n, D).cuda())      # no rotation
+    for layer in range(2):
+        q, k, v = rnd(80, H * G, D), rnd(80, H, D), rnd(80, H, D)
+        _, kr = c.append_prefill(layer, ["a"], q, k, v, *turn(80), cu)
+        assert torch.equal(kr, k)
+    c.commit("a", 80)
+    assert c.cache_prefix(prompt, "a") == 80
+    c.allocate("b", 81, prompt + [7])
+    assert c.get_cache_len("b") == 80 and c.position("b") == 80
+    shared = c.get_block_table("b")[:5]
+    assert shared == c.get_block_table("a")[:5]
+    before = [t[shared].clone() for t in c.k_pools]
+
+    def step(names):
+        for r in names:
+            c.reserve(r, c.get_cache_len(r) + 1)
+        for layer in range(2):
+            n = len(names)
+            q, k, v = rnd(n, H * G, 1, D), rnd(n, H, 1, D), rnd(n, H, 1, D)
+            q = c.append_decode(layer, names, q, k, v, *turn(n))
+            out = c.attend(layer, names, q)
+            state = [t.cpu() for t in (c.k_pools[layer], c.v_pools[layer], c.scales[layer])]
+            lens = [c.get_cache_len(r) + 1 for r in names]
+            table = torch.full((n, 16), -1, dtype=torch.int32)
+            for i, r in enumerate(names):
+                t = c.get_block_table(r)
+                table[i, : len(t)] = _ints(t)
+            ref, size = orc.decode(q.cpu(), *state, table, lens)
+            bound, _ = kc.decode_bound(q.cpu(), state[0], state[2], ref, size, torch.float16, 0.0)
+            assert bool(((out.cpu().double() - ref).abs() <= bound).all())
+        for r in names:
+            c.commit(r, 1)
+
+    for _ in range(3):
+        step(["b", "a"])
+    free = c.get_num_free_blocks()
+    freed = c.evict(["b"], 40, sink=4, recent=8)
+    assert c.get_num_free_blocks() == free + freed and freed == 1 - 3          # five of b's six blocks are shared, three are new
+    assert c.get_cache_len("b") == 40 and c.position("b") == 83
+    assert all(torch.equal(t[shared], s) for t, s in zip(c.k_pools, before))
+    assert c.cache_prefix(prompt, "b") == 0
+    row = c.row_of("b")
+    assert bool((c.masses[0][row, :, :40] > 0).any()) and bool((c.masses[0][row, :, 40:] == 0).all())
+    for _ in range(3):
+        step(["b", "a"])
+    assert c.evict(["a", "b"], 100) == 0
+    c.release("a"); c.release("b")
+    assert c.get_num_free_blocks() == 64

@@ -1,0 +1,139 @@
+"""CPU: the C ABI of the paged 8-bit cache, refusals that need no device, the oracle against a plain form, and the cache class's bookkeeping."""
+import ctypes
+import math
+import os
+import re
+
+import pytest
+import torch
+
+import kv8_cases as kc
+from oracle import kv8_oracle as orc
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from flash_attn_v100_b200 import _lib
+    from flash_attn_v100_b200.build import build
+    build(library="kv8")
+    return _lib.library("kv8")
+
+
+def test_library_exports_every_declared_symbol(lib):
+    from flash_attn_v100_b200 import _lib
+    text = re.sub(r"/\*.*?\*/", "", open(os.path.join(ROOT, "include", "fa_b200_kv8.h")).read(), flags=re.S)
+    names = set(re.findall(r"\b(fak_[a-z0-9_]+)\s*\(", text))
+    assert names == set(_lib.KV8_SIGNATURES) and all(hasattr(lib, n) for n in names)
+
+
+def _cache(**kw):
+    from flash_attn_v100_b200 import _lib
+    return _lib.Kv8Cache(**dict(dict(k=256, v=256, scale=256, pages=4, heads=2, dim=64, codes=0, table=256, width=2, max_pages=2), **kw))
+
+
+def test_refusals_before_the_device(lib):
+    p = ctypes.c_void_p(256)
+    ref = ctypes.byref
+    append = lambda c, k=p, stride=128, dtype=0, cu=None, batch=1, total=1: lib.fak_append_paged(ref(c), k, p, stride, stride, dtype, None, cu, batch, total, None)
+    assert append(_cache(k=None)) == -1 and b"null" in lib.fak_last_error()
+    assert append(_cache(dim=80)) == -2 and b"not built" in lib.fak_last_error()
+    for bad in (dict(codes=2), dict(pages=0), dict(heads=0), dict(width=1), dict(max_pages=0), dict(k=260), dict(scale=260)):
+        assert append(_cache(**bad)) == -1, bad
+    assert append(_cache(), dtype=2) == -1 and append(_cache(), stride=120) == -1 and append(_cache(), stride=130) == -1
+    assert append(_cache(), total=2) == -1 and append(_cache(), total=-1, cu=p) == -1
+    assert append(_cache(), k=ctypes.c_void_p(264)) == -1 and append(_cache(), k=None) == -1
+    assert append(_cache(), total=0, batch=0) == 0
+    decode = lambda c, q_heads=4, tokens=1, cap=0.0, mass=None, rows=0, cap_m=0, ws=p, n=1 << 40, dtype=0: lib.fak_decode_paged(
+        ref(c), p, p, p, 1, q_heads, tokens, dtype, cap, mass, None, rows, cap_m, ws, n, None)
+    for bad in (dict(q_heads=3), dict(q_heads=0), dict(tokens=0), dict(cap=-1.0), dict(cap=math.inf), dict(cap=math.nan), dict(mass=p), dict(ws=None), dict(n=16),
+                dict(dtype=7), dict(ws=ctypes.c_void_p(264)), dict(tokens=65536)):
+        assert decode(_cache(), **bad) == -1, bad
+    assert b"query rows" in lib.fak_last_error()
+    assert lib.fak_decode_workspace(ref(_cache()), 1, 3, 1, 0) == 0
+    assert 0 < lib.fak_decode_workspace(ref(_cache()), 1, 4, 1, 0) < lib.fak_decode_workspace(ref(_cache()), 1, 4, 1, 1)
+    evict = lambda c=_cache(), rows=1, width=1, budget=16, sink=0, recent=0, mass=p: lib.fak_evict_paged(
+        ref(c), mass, None, rows, 32, p, 1, p, width, budget, sink, recent, p, p, p, None)
+    for bad in (dict(budget=0), dict(budget=17), dict(sink=9, recent=8), dict(sink=-1), dict(rows=0), dict(mass=None)):
+        assert evict(**bad) == -1, bad
+
+
+def test_python_refusals():
+    import flash_attn_v100_b200 as fa
+    k8, v8, scale = kc.cache(2, 1, 64, torch.int8, 0)
+    table, n = torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    q = torch.zeros(1, 1, 1, 64).half()
+    with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+        fa.forward_paged_decode_gqa_kv8(q, k8, v8, scale, table, n, 1)
+    with pytest.raises(RuntimeError, match="must be CUDA tensors"):
+        fa.append_paged_kv8(q, q, k8, v8, scale, table, n, 1)
+    with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+        fa.evict_paged_kv8(torch.zeros(1, 1, 16), k8, v8, scale, table, n, 1, table, 16)
+    with pytest.raises(RuntimeError, match="must be a tensor"):
+        fa.forward_paged_decode_gqa_kv8(None, k8, v8, scale, table, n, 1)
+
+
+@pytest.mark.parametrize("codes", kc.CODES)
+def test_oracle_append_is_near_the_rows(codes):
+    """Every value comes back within half a step of its page's scale (a step and a half where codes were rounded again)."""
+    table, _ = kc.tables([45, 20], 6, 1)
+    state = kc.cache(6, 2, 64, codes, 2)
+    g = torch.Generator().manual_seed(3)
+    k, v = torch.randn(50, 2, 64, generator=g), torch.randn(50, 2, 64, generator=g)
+    orc.append(k[:40], v[:40], *state, table, None, torch.tensor([0, 30, 40], dtype=torch.int32))
+    orc.append(k[40:], v[40:], *state, table, torch.tensor([30, 10], dtype=torch.int32), torch.tensor([0, 5, 10], dtype=torch.int32))
+    want = torch.cat((k[:30], k[40:45]))
+    for h in range(2):
+        got = orc.rows_of(state[0], state[2], 0, table[0], h, 35)
+        a = want[:, h].double()
+        if codes == torch.int8:
+            limit = torch.full_like(a, 1.5 * float(state[2][table[0, :3].long(), h, 0].max()))
+        else:
+            limit = a.abs() * 2.0 ** -3 + 1e-3
+        assert bool(((got - a).abs() <= limit).all())
+
+
+def test_oracle_chooses_as_a_sort_does():
+    g = torch.Generator().manual_seed(4)
+    for n, budget, sink, recent in ((50, 20, 3, 5), (20, 20, 0, 0), (21, 20, 20, 0), (9, 1, 0, 0)):
+        mass = torch.randint(0, 5, (n,), generator=g).float()
+        got = orc.choose(mass.tolist(), n, budget, sink, recent)
+        assert len(got) == min(n, budget) and got == sorted(set(got))
+        if n > budget:
+            assert set(range(sink)) <= set(got) and set(range(n - recent, n)) <= set(got)
+            left = [i for i in range(sink, n - recent) if i not in got]
+            taken = [i for i in range(sink, n - recent) if i in got]
+            assert all((mass[i], -i) > (mass[j], -j) for i in taken for j in left)
+    assert orc.choose([0.0, math.nan, 3.0, -0.0], 4, 2, 0, 0) == [1, 2]
+    assert orc.choose([-0.0, 0.0, 0.0], 3, 1, 0, 0) == [0]
+
+
+def test_cache_class_bookkeeping():
+    from flash_attn_v100_b200 import PagedKVCache8
+    c = PagedKVCache8(8, 1, 2, 64, max_batch=2, max_blocks_per_seq=4, device="cpu", codes=torch.float8_e4m3fn)
+    assert c.k_pools[0].dtype == torch.float8_e4m3fn and c.scales[0].shape == (8, 2, 2) and c.masses[0].shape == (2, 2, 64)
+    c.masses[0].fill_(1.0)
+    row = c.allocate("a", 20)
+    assert bool((c.masses[0][row] == 0).all())
+    c.commit("a", 20)
+    assert c.position("a") == c.get_cache_len("a") == 20
+    assert c.evict(["a"], 20, 0, 0) == 0                          # nothing to cut: no kernel
+    for bad in ((0, 0, 0), (10, 6, 5), (10, -1, 0)):
+        with pytest.raises(ValueError):
+            c.evict(["a"], *bad)
+    with pytest.raises(ValueError, match="twice"):
+        c.evict(["a", "a"], 10, 0, 0)
+    c.allocate("b", 64)
+    free = c.get_num_free_blocks()
+    c.commit("b", 64)
+    with pytest.raises(MemoryError):
+        c.evict(["b"], 60, 0, 0)                                  # four new blocks are needed
+    assert c.get_num_free_blocks() == free and c.get_cache_len("b") == 64
+    c.release("a")
+    with pytest.raises(KeyError):
+        c.position("a")
+    with pytest.raises(RuntimeError, match="no sums"):
+        PagedKVCache8(8, 1, 2, 64, 2, 4, device="cpu", eviction=False).evict([], 10)
+    with pytest.raises(ValueError):
+        PagedKVCache8(8, 1, 2, 64, 2, 4, device="cpu", codes=torch.uint8)
