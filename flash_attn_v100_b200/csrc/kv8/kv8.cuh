@@ -45,6 +45,7 @@ struct DecodeArgs {
   const int* mass_index;
   int mass_rows, mass_cap;
   int n_cta, blocks;            // blocks: row blocks of a KV head
+  bool even;                    // cut evenly over all warps
   int *plan;                    // [kPlanHead + batch + 1]
   float *part, *part_ml;        // [slots][row block][dim], [slots][row block][2]
   float *scores, *lse;          // [batch, heads, blocks, max tokens, score columns], [batch, heads, rows]

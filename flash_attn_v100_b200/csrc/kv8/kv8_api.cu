@@ -48,11 +48,11 @@ int make_cache(const FakCache* p, k8::Cache& c) {
   return FAK_OK;
 }
 
-// Sequences of one launch of a decode: their running sum of pages has to fit in shared memory and in 31 bits, and heads are the grid's second dimension.
-int64_t slab_of(const FakCache* p) {
+// Sequences of one launch of a decode: their running sum of pages has to fit in shared memory, and the pages of all heads and row blocks, with what a segment
+// costs beside them, in 31 bits.
+int64_t slab_of(const FakCache* p, int blocks) {
   int64_t n = k8::kMaxBatch;
-  if (n > 65535 / p->heads) n = 65535 / p->heads;
-  const int64_t by_pages = ((1ll << 31) - 1) / p->max_pages;
+  const int64_t by_pages = ((1ll << 31) - 1) / (((int64_t)p->max_pages + 16) * p->heads * blocks);
   if (n > by_pages) n = by_pages;
   return n < 1 ? 1 : n;
 }
@@ -121,7 +121,7 @@ size_t fak_decode_workspace(const FakCache* cache, int batch, int q_heads, int t
   if (check_decode(cache, batch, q_heads, tokens) != FAK_OK || batch == 0) return 0;
   const int rows = q_heads / cache->heads * tokens;
   const k8::DecodeShape d = k8::decode_shape(cache->dim, rows, sm_count());
-  const int64_t slab = slab_of(cache);
+  const int64_t slab = slab_of(cache, d.blocks);
   return layout_of(cache, batch < slab ? batch : slab, rows, with_mass != 0, d).bytes;
 }
 
@@ -138,11 +138,11 @@ int fak_decode_paged(const FakCache* cache, const void* q, void* out, const int3
              mass_cap);
   const int rows = q_heads / cache->heads * tokens;
   const k8::DecodeShape d = k8::decode_shape(cache->dim, rows, sm_count());
-  const int64_t slab = batch < slab_of(cache) ? batch : slab_of(cache);
+  const int64_t slab = batch < slab_of(cache, d.blocks) ? batch : slab_of(cache, d.blocks);
   const Layout w = layout_of(cache, slab, rows, mass != nullptr, d);
   FA_REQUIRE(workspace_bytes >= w.bytes, "the workspace has %zu bytes, %zu are needed", workspace_bytes, w.bytes);
-  FA_REQUIRE((int64_t)cache->heads * d.blocks * slab < (1ll << 30) &&
-                 ((double)slab * cache->max_pages * cache->heads * d.blocks / d.n_cta < 2e9), "too many pages: %lld sequences of %d", (long long)slab, cache->max_pages);
+  FA_REQUIRE(((int64_t)cache->max_pages + 16) * cache->heads * d.blocks < (1ll << 31), "too many pages: %d of a sequence, %d heads, %d row blocks", cache->max_pages,
+             cache->heads, d.blocks);
   k8::DecodeArgs a{};
   if ((rc = make_cache(cache, a.c)) != FAK_OK) return rc;
   uint8_t* base = static_cast<uint8_t*>(workspace);

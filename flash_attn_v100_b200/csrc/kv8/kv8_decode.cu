@@ -5,13 +5,19 @@
 // with one scale ks, vs for the 16 tokens of a page and head.  Bound by HBM (2 D bytes a token and KV head against 4 D flop a row), so the
 // rows of a KV head (its query heads times the new tokens) share every code that is read, in blocks of 8 or 16.  Keys, and then output dimensions,
 // are the 16 rows of mma.sync.m16n8k16 and the query rows its 8 columns: S^T = K Q^T, O^T = V^T P^T.
-// Codes go from global memory straight to registers in the operands' layout: a lane's 16 bytes of a key row are four steps of the (permuted)
-// contraction, and its 16 bytes of four tokens' values the rows of eight tiles of O^T.  They become fp16 there, exactly.
+// A warp copies pages to a ring of its own in shared memory (cp.async, 16 bytes a lane, the pieces of a row placed so that the reads meet no bank twice) and
+// runs ahead of its own reads from one piece into the next.  A lane's 16 bytes of a key row are four steps of the (permuted) contraction, and its 16
+// bytes of four tokens' values the rows of eight tiles of O^T.  They become fp16 in registers, exactly.
 // K's scale multiplies the finished scores.  V's scale goes into the exponent: with m the running maximum of s + log2 vs the weight that meets the
 // codes is 2^(s + log2 vs - m) <= 1, so fp16 keeps 11 bits of the products that matter whatever the pages' scales are; the sum of weights
 // takes 2^(s - m) in fp32.
-// The pages of all sequences and heads are cut evenly over the CTAs; where there are fewer segments than half the CTAs each is cut into equal
-// parts, at least kLeastPart pages.  Parts of a cut segment go through global memory to a second launch.
+// The pages of all sequences and heads are cut evenly over the warps; where there are fewer segments than half the CTAs each is cut into equal
+// parts, at least kLeastPart pages, that the warps of a CTA share.  Parts of a cut segment go through global memory to a second launch, which, like the
+// first, is on its way before the launch in front of it has ended.
+// Measured: 64 sequences of 512 to 8192 tokens, 32 heads on 8 of 128, int8: 108.5 us for 573 MB, 5.3 TB/s (124 with loads straight to registers and an
+// even cut over CTAs).  Of it 8 us pass before the first codes are there, and the warps end between 65 and 98 us: some SMs get their bytes
+// a sixth later than others.  Looked at and left: L2 prefetches 2 to 6 steps ahead (slower by 5 to 14 %: nothing waits for DRAM alone), ranges for early
+// finishers, as CTAs of their own or taken over by running ones (the longer program costs what they gain), more CTAs than fit at once (12 us a wave).
 #include <math_constants.h>
 
 #include "kv8.cuh"
@@ -22,6 +28,8 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kLeastPart = 8;
+constexpr int kOpening = 4;
+
 
 __device__ __forceinline__ float log2_of(float x) {
   float y;
@@ -71,12 +79,10 @@ __device__ __forceinline__ int pages_of(const DecodeArgs& a, int b) {
 }
 __device__ __forceinline__ int len_of(const DecodeArgs& a, int b) { return min(max(a.lens[b], 0), a.c.max_pages * kPage); }
 
-// How the pages are cut.  even: CTA c takes the pages [c * per, (c + 1) * per) of all segments in order.  else: every segment of sequence b has
-// ceil(pages / per) parts, and CTA c takes one.  first[b]: pages (parts) of a KV head and row block before sequence b.
+// How the pages are cut.  even: unit u (a warp) takes `per` of all segments' places in order, from u * per on; a segment has kOpening places that stand for what a piece costs apart from its pages, then one for each page.  else: every
+// segment of sequence b has ceil(pages / per) parts, and unit u (a CTA) takes one.  first[b]: places (parts) of a KV head and row block before sequence b.
 struct Plan {
-  bool even;
   int per;
-  const int* first;
 };
 
 // Running sums of f(b) in first[0 .. batch], by the whole block; returns their total.
@@ -92,7 +98,6 @@ __device__ __forceinline__ int running_sum(int batch, int* first, int* warp_sums
     const int y = __shfl_up_sync(0xffffffffu, x, d);
     if (lane >= d) x += y;
   }
-  __syncthreads();
   if (lane == 31) warp_sums[w] = x;
   __syncthreads();
   int at = x - sum, total = 0;
@@ -110,97 +115,248 @@ __device__ __forceinline__ int running_sum(int batch, int* first, int* warp_sums
   return total;
 }
 
-__device__ __forceinline__ Plan make_plan(const DecodeArgs& a, int* first, int* warp_sums) {
+__device__ __forceinline__ Plan make_plan(const DecodeArgs& a, int* first, int* lens, int* warp_sums) {
   Plan p;
   const int lanes = a.c.heads * a.blocks, segments = a.batch * lanes;
-  const int64_t units = (int64_t)running_sum(a.batch, first, warp_sums, [&](int b) { return pages_of(a, b); }) * lanes;
-  p.even = 2 * segments > a.n_cta;
-  p.first = first;
-  if (p.even) {
-    p.per = max(1, (int)((units + a.n_cta - 1) / a.n_cta));
+  for (int b = threadIdx.x; b < a.batch; b += kThreads) lens[b] = min(max(a.lens[b], 0), a.c.max_pages * kPage);
+  __syncthreads();
+  const int opening = a.even ? kOpening : 0;
+  const int units = running_sum(a.batch, first, warp_sums, [&](int b) { return lens[b] ? (lens[b] + kPage - 1) / kPage + opening : 0; }) * lanes;
+  if (a.even) {
+    const int warps = a.n_cta * kWarps;
+    p.per = max(1, (units + warps - 1) / warps);
   } else {
     // no more parts than CTAs: sum of ceil(pages / per) <= units / per + segments
-    p.per = max(kLeastPart, (int)((units + a.n_cta - segments - 1) / (a.n_cta - segments)));
-    running_sum(a.batch, first, warp_sums, [&](int b) { return (pages_of(a, b) + p.per - 1) / p.per; });
+    p.per = max(kLeastPart, (units + a.n_cta - segments - 1) / (a.n_cta - segments));
+    running_sum(a.batch, first, warp_sums + kWarps, [&](int b) { return ((lens[b] + kPage - 1) / kPage + p.per - 1) / p.per; });
   }
   return p;
 }
 
+// What the second launch needs to know of a row: reference and sum of a part, or the logarithm of a whole row's sum for its keys' weights.
+__device__ __forceinline__ void leave_sums(const DecodeArgs& a, bool whole, int64_t slot, int64_t head, int row, int r, int row_block, float m, float l) {
+  if (!whole) *reinterpret_cast<float2*>(a.part_ml + (slot * row_block + r) * 2) = make_float2(m, l);
+  else if (a.lse != nullptr) a.lse[head * a.rows + row] = l == 0.f ? CUDART_INF_F : m + log2f(l);
+}
+
 // The last b with first[b] * lanes <= x that is not empty (there is one).
-__device__ __forceinline__ int find(const int* first, int batch, int64_t x, int lanes) {
+__device__ __forceinline__ int find(const int* first, int batch, int x, int lanes) {
   int lo = 0, hi = batch;
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
-    if ((int64_t)first[mid] * lanes <= x) lo = mid; else hi = mid;
+    if (first[mid] * lanes <= x) lo = mid; else hi = mid;
   }
   return lo;
 }
 
-template <int D, int NT, bool E4M3>
+template <int D, int NT>
 struct Shape {
   static constexpr int kTile = D == 256 || (D == 128 && NT == 2) ? 1 : 2;      // pages of a warp's step
+  static constexpr int kSlots = D == 128 && NT == 1 ? 2 : 3;     // steps whose codes are under way or in use
   static constexpr int kChunks = D / 64;       // 16-byte pieces of a key row that a lane takes
   static constexpr int kSteps = D / 16;        // of the contraction, and tiles of O^T
   static constexpr int kRows = NT * 8;
   static constexpr int kCtas = D == 256 ? 2 : NT == 2 ? (D == 64 ? 3 : 2) : (D == 64 ? 4 : 3);
+  static constexpr int kRing = kSlots * kTile * (2 * kPage * D + 8);      // bytes of a warp
+  static constexpr int kMerge = kRows * (D + 4 + 2) * 4;            // what a warp hands over at the end of a shared piece, in the same place
+  static constexpr int kWarpBytes = ((kRing > kMerge ? kRing : kMerge) + 127) / 128 * 128;
 };
 
+// Where 16-byte piece `chunk` of a row lies in a page's tile of shared memory, so that the eight lanes of a phase meet eight banks' groups: keys are read by rows
+// g, g + 1 and pieces 0 to 3, values by rows 0, 2, 4, 6 (+ 1) and two pieces (D = 64: halves of one).
+template <int D>
+__device__ __forceinline__ int key_at(int row, int chunk) {
+  return row * D + ((D >= 128 ? chunk ^ ((row & 1) << 2) : chunk) << 4);
+}
+template <int D>
+__device__ __forceinline__ int value_at(int row, int chunk) {
+  if constexpr (D == 64) return (row >> 1) * 128 + ((((row & 1) << 2 | chunk) ^ (row & 6)) << 4);
+  if constexpr (D == 128) return row * D + ((chunk ^ (row & 6)) << 4);
+  return row * D + ((chunk ^ ((row >> 1 & 1) | (row & 4))) << 4);
+}
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at));
+  return r;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t at) {
+  uint2 r;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(at));
+  return r;
+}
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+
 template <int D, int NT, bool E4M3>
-__global__ void __launch_bounds__(kThreads, Shape<D, NT, E4M3>::kCtas) decode_kernel(const DecodeArgs a) {
-  using S = Shape<D, NT, E4M3>;
-  constexpr int kTile = S::kTile, kChunks = S::kChunks, kSteps = S::kSteps, kRows = S::kRows;
-  extern __shared__ int smem[];
-  int* first = smem;                                              // [batch + 1]
-  float* sm_o = reinterpret_cast<float*>(smem + ((a.batch + 1 + 3) & ~3));      // [kWarps][kRows][D + 4]
-  float* sm_ml = sm_o + kWarps * kRows * (D + 4);                 // [kWarps][kRows][2]
-  __shared__ int warp_sums[kWarps];
+__global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(const DecodeArgs a) {
+  using S = Shape<D, NT>;
+  constexpr int kTile = S::kTile, kSlots = S::kSlots, kChunks = S::kChunks, kSteps = S::kSteps, kRows = S::kRows;
+  extern __shared__ __align__(128) int smem[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>(smem);               // [kWarps][kWarpBytes]
+  int* first = smem + kWarps * S::kWarpBytes / 4;                 // [batch + 1]
+  int* lens = first + a.batch + 1;                                // [batch]
+  const auto sm_o = [&](int w) { return reinterpret_cast<float*>(ring + w * S::kWarpBytes); };      // [kRows][D + 4]
+  const auto sm_ml = [&](int w) { return sm_o(w) + kRows * (D + 4); };                              // [kRows][2]
+  __shared__ int warp_sums[2 * kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int lanes = a.c.heads * a.blocks;
-  const Plan plan = make_plan(a, first, warp_sums);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Plan plan = make_plan(a, first, lens, warp_sums);
   if (blockIdx.x == 0) {
     for (int i = tid; i <= a.batch; i += kThreads) a.plan[kPlanHead + i] = first[i];
-    if (tid == 0) {
-      a.plan[0] = plan.even;
-      a.plan[1] = plan.per;
-    }
+    if (tid == 0) a.plan[0] = plan.per;
   }
   // Sequences without keys.
   for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
-    if (pages_of(a, b) != 0) continue;
+    if (lens[b] != 0) continue;
     const int64_t n = (int64_t)a.c.heads * a.rows * D;
     uint16_t* o = static_cast<uint16_t*>(a.out) + b * n;
     for (int64_t i = tid; i < n; i += kThreads) o[i] = 0;
   }
-  int64_t at = plan.even ? (int64_t)blockIdx.x * plan.per : blockIdx.x;
-  int64_t end = (int64_t)first[a.batch] * lanes;
-  end = plan.even ? min(end, at + plan.per) : min(end, at + 1);
-  const int64_t range0 = at;
-  while (at < end) {
-    // ---- the piece: pages [p0, p1) of sequence b, KV head h, rows from r0 on
-    const int b = find(first, a.batch, at, lanes);
-    const int pages = pages_of(a, b), parts = first[b + 1] - first[b];
-    const int64_t in = at - (int64_t)first[b] * lanes;
-    int h, rb, p0, p1;
-    int64_t slot;
-    if (plan.even) {
-      const int seg = (int)(in / pages);
-      h = seg / a.blocks;
-      rb = seg % a.blocks;
-      p0 = (int)(in % pages);
-      p1 = (int)min((int64_t)pages, p0 + (end - at));
-      slot = 2 * (int64_t)blockIdx.x + (at == range0 ? 0 : 1);
-      at += p1 - p0;
+  // even: every warp has a range of its own.  else: the warps of a CTA share its part.
+  const int unit = a.even ? blockIdx.x * kWarps + warp : blockIdx.x;
+  const int share = a.even ? 1 : kWarps, turn = a.even ? 0 : warp;
+  const int total = first[a.batch] * lanes, range0 = a.even ? unit * plan.per : unit;
+  const int end = min(total, a.even ? range0 + plan.per : unit + 1);
+
+  // A piece: the pages [p0, p1) of one sequence, KV head and row block.  The warp takes it in steps: pages p0 + (turn + share * i) * kTile + {0 .. kTile - 1}.
+  struct Piece {
+    int b, h, rb, p0, p1, pages, next, steps;
+  };
+  const auto locate = [&](int at) {
+    Piece x;
+    x.b = find(first, a.batch, at, lanes);
+    x.pages = (lens[x.b] + kPage - 1) / kPage;
+    const int in = at - first[x.b] * lanes;
+    if (a.even) {
+      const int places = x.pages + kOpening, seg = in / places, before = in - seg * places;
+      x.h = seg / a.blocks;
+      x.rb = seg - x.h * a.blocks;
+      x.next = min(end, at + places - before);
+      x.p0 = max(0, before - kOpening);
+      x.p1 = before + x.next - at - kOpening;      // (<= p0: the range ends before the first page)
     } else {
-      rb = (int)(in % a.blocks);
-      h = (int)(in / a.blocks / parts);
-      const int part = (int)(in / a.blocks % parts);
-      p0 = (int)((int64_t)pages * part / parts);
-      p1 = (int)((int64_t)pages * (part + 1) / parts);
-      slot = blockIdx.x;
-      at = end;
+      const int parts = first[x.b + 1] - first[x.b], i = in / a.blocks;
+      x.rb = in - i * a.blocks;
+      x.h = i / parts;
+      const int part = i - x.h * parts;
+      x.p0 = (int)((int64_t)x.pages * part / parts);
+      x.p1 = (int)((int64_t)x.pages * (part + 1) / parts);
+      x.next = end;
     }
-    const bool whole = p0 == 0 && p1 == pages;
-    const int len = len_of(a, b), r0 = rb * kRows, rows = min(kRows, a.rows - r0);
+    x.steps = (max(0, x.p1 - x.p0 + kTile - 1) / kTile - turn + share - 1) / share;
+    return x;
+  };
+
+  // The ring: slot s has the keys of kTile pages, their values and, behind all slots, their scales.  What fills it runs kSlots steps ahead of what reads it, from one
+  // piece into the next.  A lane copies 16 bytes of every 512, and holds the number of one of the next 32 pages.
+  constexpr int kAhead = 32 / kTile;
+  constexpr int kPageBytes = kPage * D, kCopies = kPageBytes / 512, kLanesRow = D / 16;
+  const int64_t page_bytes = (int64_t)a.c.heads * kPageBytes;
+  const uint32_t mine_at = smem_u32(ring + warp * S::kWarpBytes), scales_at = mine_at + kSlots * 2 * kTile * kPageBytes;
+  Piece f;                                      // the piece that is being copied
+  int f_i = 0, f_at = range0, f_id = 0, f_id_next = 0, pg[kTile];
+  const int* f_table = nullptr;
+  f.steps = 0;
+  const auto page_numbers = [&](int i0) {       // of the steps i0 .. i0 + kAhead - 1
+    const int p = f.p0 + (turn + share * (i0 + lane / kTile)) * kTile + lane % kTile;
+    return p < f.p1 ? f_table[p] : 0;
+  };
+  const auto open = [&] {                       // (only the last piece of a range can be without pages: it then ends the range)
+    f = locate(f_at);
+    f_at = f.next;
+    f_i = 0;
+    if (f.steps <= 0) return;
+    f_table = a.c.table + (int64_t)f.b * a.c.width;
+    f_id = page_numbers(0);
+    if (f.steps > kAhead) f_id_next = page_numbers(kAhead);
+    const int64_t q0 = (((int64_t)f.b * a.c.heads + f.h) * a.rows + f.rb * kRows) * D;      // (the rows of a KV head, in lines of 64 elements)
+    if (lane < min(kRows, a.rows - f.rb * kRows) * (D / 64))
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint16_t*>(a.q) + q0 + lane * 64));
+  };
+  const auto copy_keys = [&](int slot) {
+    if (f_i < f.steps) {
+      const int base = f.p0 + (turn + share * f_i) * kTile;
+#pragma unroll
+      for (int u = 0; u < kTile; ++u) {
+        pg[u] = __shfl_sync(0xffffffffu, f_id, f_i % kAhead * kTile + u);
+        if (base + u < f.p1) {
+          const bool fine = page_ok(a.c, pg[u]);
+          if (!fine) pg[u] = 0;
+          const uint8_t* from = a.c.k + pg[u] * page_bytes + f.h * kPageBytes + lane * 16;
+#pragma unroll
+          for (int c = 0; c < kCopies; ++c)
+            copy16(mine_at + (slot * 2 * kTile + u) * kPageBytes + key_at<D>(c * (32 / kLanesRow) + lane / kLanesRow, lane % kLanesRow), from + c * 512);
+          if (lane == u) {
+            const uint32_t to = scales_at + (slot * kTile + u) * 8;
+            if (fine) {
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(a.c.scale + ((int64_t)pg[u] * a.c.heads + f.h) * 2) : "memory");
+            } else {
+              atomicOr(a.c.status, kStatusBadPageId);
+              asm volatile("st.shared.v2.f32 [%0], {%1, %1};" ::"r"(to), "f"(CUDART_NAN_F) : "memory");
+            }
+          }
+        }
+      }
+    }
+    cp_async_commit();
+  };
+  const auto copy_values = [&](int slot) {
+    if (f_i < f.steps) {
+      const int base = f.p0 + (turn + share * f_i) * kTile;
+#pragma unroll
+      for (int u = 0; u < kTile; ++u)
+        if (base + u < f.p1) {
+          const uint8_t* from = a.c.v + pg[u] * page_bytes + f.h * kPageBytes + lane * 16;
+#pragma unroll
+          for (int c = 0; c < kCopies; ++c)
+            copy16(mine_at + ((slot * 2 + 1) * kTile + u) * kPageBytes + value_at<D>(c * (32 / kLanesRow) + lane / kLanesRow, lane % kLanesRow), from + c * 512);
+        }
+      ++f_i;
+      if (f_i == f.steps) {
+        if (f_at < end) open();
+      } else if (f_i % kAhead == 0) {
+        f_id = f_id_next;
+        if (f_i + kAhead < f.steps) f_id_next = page_numbers(f_i + kAhead);
+      }
+    }
+    cp_async_commit();
+  };
+  // Query rows of a piece as they are, a lane's 16 columns of 64 of row g (and g + 8).
+  uint4 raw_q[NT][kChunks][2];
+  const auto load_q = [&](const Piece& x) {
+    const int r0 = x.rb * kRows, last = min(kRows, a.rows - r0) - 1;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const uint16_t* q = static_cast<const uint16_t*>(a.q) + (((int64_t)x.b * a.c.heads + x.h) * a.rows + r0 + min(n * 8 + g, last)) * D;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) raw_q[n][c][i] = *reinterpret_cast<const uint4*>(q + (c * 4 + t) * 16 + i * 8);
+    }
+  };
+  Piece x;
+  int at = range0;
+  if (at < end) {
+    open();
+    x = locate(at);
+    load_q(x);
+#pragma unroll 1                                // (a longer program starts later)
+    for (int i = 0; i < kSlots; ++i) {
+      copy_keys(i);
+      copy_values(i);
+    }
+  }
+  int at_slot = 0;
+  while (at < end) {
+    const int b = x.b, h = x.h, rb = x.rb, p0 = x.p0, p1 = x.p1, len = lens[b];
+    const int64_t slot = a.even ? 2 * unit + (at == range0 ? 0 : 1) : unit;
+    at = x.next;
+    if (a.even && p1 <= p0) break;
+    const bool whole = p0 == 0 && p1 == x.pages;
+    const int r0 = rb * kRows, rows = min(kRows, a.rows - r0);
     const int64_t head = (int64_t)b * a.c.heads + h;
     // ---- query rows as the second operand, fp16; bf16 rows are brought into its range by a power of two
     uint32_t qf[NT][kSteps][2];
@@ -208,17 +364,15 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT, E4M3>::kCtas) decode_ke
     int limit[NT][2];                           // keys that they see
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int r = n * 8 + g;
-      const uint16_t* q = static_cast<const uint16_t*>(a.q) + (head * a.rows + r0 + min(r, rows - 1)) * D;
       float sum = 0.f, up = 1.f;
       uint32_t raw[kSteps][2];
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        const uint4 x0 = *reinterpret_cast<const uint4*>(q + (c * 4 + t) * 16), x1 = *reinterpret_cast<const uint4*>(q + (c * 4 + t) * 16 + 8);
-        const uint32_t w[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+      for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) raw[c * 4 + i / 2][i & 1] = w[i];
-      }
+        for (int i = 0; i < 2; ++i) {
+          raw[c * 4 + i * 2][0] = raw_q[n][c][i].x; raw[c * 4 + i * 2][1] = raw_q[n][c][i].y;
+          raw[c * 4 + i * 2 + 1][0] = raw_q[n][c][i].z; raw[c * 4 + i * 2 + 1][1] = raw_q[n][c][i].w;
+        }
       if (a.bf16) {
         uint32_t most = 0;
 #pragma unroll
@@ -268,81 +422,17 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT, E4M3>::kCtas) decode_ke
       l[n][0] = l[n][1] = 0.f;
     }
 
-    // ---- the warp's steps: pages p0 + (warp + kWarps * i) * kTile + {0 .. kTile - 1}
-    const int steps = (p1 - p0 + kTile - 1) / kTile;
-    const int mine = (steps - warp + kWarps - 1) / kWarps;      // <= 0: none
-    constexpr int kAhead = 32 / kTile;                          // steps whose pages a warp looks up at once, a lane each
-    int id_next = 0, id = 0;
-    float2 sc_next = make_float2(0.f, 0.f), sc = sc_next;
-    const auto look_up = [&](int i0) {                          // pages of the steps i0 .. i0 + kAhead - 1
-      const int p = p0 + (warp + kWarps * (i0 + lane / kTile)) * kTile + lane % kTile;
-      id_next = 0;
-      sc_next = make_float2(0.f, 0.f);
-      if (p < p1) {
-        id_next = a.c.table[(int64_t)b * a.c.width + p];
-        const bool fine = page_ok(a.c, id_next);
-        if (!fine) {
-          atomicOr(a.c.status, kStatusBadPageId);
-          id_next = 0;
-        }
-        sc_next = *reinterpret_cast<const float2*>(a.c.scale + ((int64_t)id_next * a.c.heads + h) * 2);
-        // a scale that is not finite spoils what sees the page, whatever the codes
-        if (!fine || !(fabsf(sc_next.x) <= 3.4028235e38f)) sc_next.x = CUDART_NAN_F;
-        sc_next.y = log2_of(sc_next.y);
-      }
-    };
-    const int64_t page_bytes = (int64_t)a.c.heads * kPage * D;
-    const uint8_t* kbase = a.c.k + (int64_t)h * kPage * D + g * D + t * 16;
-    const uint8_t* vbase = a.c.v + (int64_t)h * kPage * D + 2 * t * D + g * (D / 8);
-    uint32_t kr[kTile][2][kChunks][4];          // key rows g and g + 8
-    uint32_t vr[kTile][4][D / 32];              // value rows 2t, 2t + 1, 2t + 8, 2t + 9
-    const auto load_keys = [&](const int (&pg)[kTile]) {
-#pragma unroll
-      for (int u = 0; u < kTile; ++u)
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c) {
-            const uint4 x = load_stream16(kbase + pg[u] * page_bytes + half * 8 * D + c * 64);
-            kr[u][half][c][0] = x.x; kr[u][half][c][1] = x.y; kr[u][half][c][2] = x.z; kr[u][half][c][3] = x.w;
-          }
-    };
-    const auto load_values = [&](const int (&pg)[kTile]) {
-#pragma unroll
-      for (int u = 0; u < kTile; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const uint8_t* p = vbase + pg[u] * page_bytes + ((r & 1) + (r >> 1) * 8) * D;
-          if constexpr (D == 64) {
-            const uint2 x = load_stream8(p);
-            vr[u][r][0] = x.x; vr[u][r][1] = x.y;
-          } else {
-#pragma unroll
-            for (int c = 0; c < D / 128; ++c) {
-              const uint4 x = load_stream16(p + c * 16);
-              vr[u][r][c * 4] = x.x; vr[u][r][c * 4 + 1] = x.y; vr[u][r][c * 4 + 2] = x.z; vr[u][r][c * 4 + 3] = x.w;
-            }
-          }
-        }
-    };
-    int pg[kTile];                              // pages of the step whose loads come next
-    if (mine > 0) {
-      look_up(0);
-      id = id_next;
-      sc = sc_next;
-      if (mine > kAhead) look_up(kAhead);
-#pragma unroll
-      for (int u = 0; u < kTile; ++u) pg[u] = __shfl_sync(0xffffffffu, id, u);
-      load_keys(pg);
-      load_values(pg);
-    }
-    for (int i = 0; i < mine; ++i) {
-      const int base = p0 + (warp + kWarps * i) * kTile, j = i % kAhead;
+    for (int i = 0; i < x.steps; ++i) {
+      const int base = p0 + (turn + share * i) * kTile;
+      cp_async_wait<2 * kSlots - 1>();
+      __syncwarp();
       float ks[kTile], lv[kTile];
 #pragma unroll
       for (int u = 0; u < kTile; ++u) {
-        ks[u] = __shfl_sync(0xffffffffu, sc.x, j * kTile + u);
-        lv[u] = __shfl_sync(0xffffffffu, sc.y, j * kTile + u);
+        float vs;
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(ks[u]), "=f"(vs) : "r"(scales_at + (at_slot * kTile + u) * 8));
+        if (!(fabsf(ks[u]) <= 3.4028235e38f)) ks[u] = CUDART_NAN_F;      // a scale that is not finite spoils what sees the page, whatever the codes
+        lv[u] = base + u < p1 ? log2_of(vs) : 0.f;
       }
       // ---- S^T = K Q^T
       float s[kTile][NT][4];
@@ -350,29 +440,24 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT, E4M3>::kCtas) decode_ke
       for (int u = 0; u < kTile; ++u)
 #pragma unroll
         for (int n = 0; n < NT; ++n) s[u][n][0] = s[u][n][1] = s[u][n][2] = s[u][n][3] = 0.f;
+      const uint32_t keys = mine_at + at_slot * 2 * kTile * kPageBytes, vals = keys + kTile * kPageBytes;
 #pragma unroll
       for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int u = 0; u < kTile; ++u) {
+          const uint4 x0 = lds16(keys + u * kPageBytes + key_at<D>(g, c * 4 + t)), x1 = lds16(keys + u * kPageBytes + key_at<D>(g + 8, c * 4 + t));
+          const uint32_t k0[4] = {x0.x, x0.y, x0.z, x0.w}, k1[4] = {x1.x, x1.y, x1.z, x1.w};
 #pragma unroll
-          for (int u = 0; u < kTile; ++u) {
+          for (int w = 0; w < 4; ++w) {
             uint32_t f[4];
-            key_pairs<E4M3>(kr[u][0][c][w], f[0], f[2]);
-            key_pairs<E4M3>(kr[u][1][c][w], f[1], f[3]);
+            key_pairs<E4M3>(k0[w], f[0], f[2]);
+            key_pairs<E4M3>(k1[w], f[1], f[3]);
 #pragma unroll
             for (int n = 0; n < NT; ++n) mma_f16_16816(s[u][n], f, qf[n][c * 4 + w][0], qf[n][c * 4 + w][1]);
           }
-      if (j == kAhead - 1) {
-        id = id_next;
-        sc = sc_next;
-        if (i + 1 + kAhead < mine) look_up(i + 1 + kAhead);
-      }
-      const bool more = i + 1 < mine;
-      if (more) {
-#pragma unroll
-        for (int u = 0; u < kTile; ++u) pg[u] = __shfl_sync(0xffffffffu, id, (j + 1) % kAhead * kTile + u);
-        load_keys(pg);
-      }
+        }
+      __syncwarp();
+      copy_keys(at_slot);
       // ---- scores in base 2
       const int key0 = base * kPage;
 #pragma unroll
@@ -461,46 +546,99 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT, E4M3>::kCtas) decode_ke
         }
       }
       // ---- O^T += V^T P^T
-      if (E4M3 && masked) {                     // codes behind the last key may stand for NaN
+      cp_async_wait<2 * kSlots - 1>();
+      __syncwarp();
 #pragma unroll
-        for (int u = 0; u < kTile; ++u)
+      for (int u = 0; u < kTile; ++u) {
+        uint32_t vr[4][D / 32];                 // rows 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int key = key0 + u * kPage + 2 * t + (r & 1) + (r >> 1) * 8;
-            if (key >= len || base + u >= p1)
+        for (int r = 0; r < 4; ++r) {
+          const int row = 2 * t + (r & 1) + (r >> 1) * 8;
+          if constexpr (D == 64) {
+            const uint2 x = lds8(vals + u * kPageBytes + value_at<D>(row, g >> 1) + (g & 1) * 8);
+            vr[r][0] = x.x; vr[r][1] = x.y;
+          } else {
 #pragma unroll
-              for (int w = 0; w < D / 32; ++w) vr[u][r][w] = 0;
+            for (int c = 0; c < D / 128; ++c) {
+              const uint4 x = lds16(vals + u * kPageBytes + value_at<D>(row, g * (D / 128) + c));
+              vr[r][c * 4] = x.x; vr[r][c * 4 + 1] = x.y; vr[r][c * 4 + 2] = x.z; vr[r][c * 4 + 3] = x.w;
+            }
           }
-      }
+          if (E4M3 && masked && (key0 + u * kPage + row >= len || base + u >= p1)) {      // codes behind the last key may stand for NaN
 #pragma unroll
-      for (int w = 0; w < D / 32; ++w)
+            for (int w = 0; w < D / 32; ++w) vr[r][w] = 0;
+          }
+        }
 #pragma unroll
-        for (int high = 0; high < 2; ++high)
+        for (int w = 0; w < D / 32; ++w)
 #pragma unroll
-          for (int u = 0; u < kTile; ++u) {
+          for (int high = 0; high < 2; ++high) {
             uint32_t f[4];
-            value_pairs<E4M3>(vr[u][0][w], vr[u][1][w], high, f[0], f[1]);
-            value_pairs<E4M3>(vr[u][2][w], vr[u][3][w], high, f[2], f[3]);
+            value_pairs<E4M3>(vr[0][w], vr[1][w], high, f[0], f[1]);
+            value_pairs<E4M3>(vr[2][w], vr[3][w], high, f[2], f[3]);
 #pragma unroll
             for (int n = 0; n < NT; ++n) mma_f16_16816(o[n][w * 2 + high], f, pf[u][n][0], pf[u][n][1]);
           }
-      if (more) load_values(pg);
+      }
+      __syncwarp();
+      copy_values(at_slot);
+      at_slot = at_slot + 1 == kSlots ? 0 : at_slot + 1;
     }
 
-    // ---- the warps' parts together
+    Piece next;
+    if (at < end) {                             // the next piece's rows come while this one's go out
+      next = locate(at);
+      load_q(next);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 4);
+        l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 8);
+        l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 16);
+      }
+    if (a.even) {                            // a warp's own piece: a lane has D / 8 columns of each of its rows
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int r = n * 8 + 2 * t + c;
+          if (r >= rows) continue;
+          if (whole) {
+            const float inv = l[n][c] == 0.f ? 0.f : 1.f / l[n][c];
+            uint16_t* to = static_cast<uint16_t*>(a.out) + (head * a.rows + r0 + r) * D + g * (D / 8);
+#pragma unroll
+            for (int k = 0; k < kSteps; k += 4) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w[e] = pack_out16x2(o[n][k + e][c] * inv, o[n][k + e][c + 2] * inv, a.bf16);
+              *reinterpret_cast<uint4*>(to + 2 * k) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          } else {
+            float* to = a.part + (slot * kRows + r) * D + g * (D / 8);
+#pragma unroll
+            for (int k = 0; k < kSteps; k += 2)
+              *reinterpret_cast<float4*>(to + 2 * k) = make_float4(o[n][k][c], o[n][k][c + 2], o[n][k + 1][c], o[n][k + 1][c + 2]);
+          }
+          if (g == 0) leave_sums(a, whole, slot, head, r0 + r, r, kRows, m[n][c], l[n][c]);
+        }
+      x = next;
+      continue;
+    }
+    // ---- the warps' parts together, where their rings were
+    cp_async_wait<0>();
+    __syncwarp();
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int r = n * 8 + 2 * t + c;
-        l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 4);
-        l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 8);
-        l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 16);
         if (g == 0) {
-          sm_ml[(warp * kRows + r) * 2] = m[n][c];
-          sm_ml[(warp * kRows + r) * 2 + 1] = l[n][c];
+          sm_ml(warp)[r * 2] = m[n][c];
+          sm_ml(warp)[r * 2 + 1] = l[n][c];
         }
-        float* to = sm_o + (warp * kRows + r) * (D + 4) + g * (D / 8);
+        float* to = sm_o(warp) + r * (D + 4) + g * (D / 8);
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) *reinterpret_cast<float2*>(to + 2 * k) = make_float2(o[n][k][c], o[n][k][c + 2]);
       }
@@ -509,65 +647,80 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT, E4M3>::kCtas) decode_ke
       const int r = i / (D / 4), d = i % (D / 4) * 4;
       float top = -CUDART_INF_F, sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_ml[(w * kRows + r) * 2]);
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_ml(w)[r * 2]);
       const float ref = top == -CUDART_INF_F ? 0.f : top;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = fast_exp2(sm_ml[(w * kRows + r) * 2] - ref);
-        sum += sm_ml[(w * kRows + r) * 2 + 1] * f;
-        const float4 x = *reinterpret_cast<const float4*>(sm_o + (w * kRows + r) * (D + 4) + d);
+        const float f = fast_exp2(sm_ml(w)[r * 2] - ref);
+        sum += sm_ml(w)[r * 2 + 1] * f;
+        const float4 x = *reinterpret_cast<const float4*>(sm_o(w) + r * (D + 4) + d);
         acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
       }
       if (whole) {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         uint2 packed = make_uint2(pack_out16x2(acc.x * inv, acc.y * inv, a.bf16), pack_out16x2(acc.z * inv, acc.w * inv, a.bf16));
         *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (head * a.rows + r0 + r) * D + d) = packed;
-        if (a.lse != nullptr && d == 0) a.lse[head * a.rows + r0 + r] = sum == 0.f ? CUDART_INF_F : ref + log2f(sum);
       } else {
         *reinterpret_cast<float4*>(a.part + (slot * kRows + r) * D + d) = acc;
-        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * kRows + r) * 2) = make_float2(top, sum);
       }
+      if (d == 0) leave_sums(a, whole, slot, head, r0 + r, r, kRows, top, sum);
     }
     __syncthreads();
   }
 }
 
-// The parts of a row together: a CTA for each query row of a KV head; rows of segments that were not cut have nothing to do.
-template <int D>
-__global__ void __launch_bounds__(kThreads) merge_kernel(const DecodeArgs a, int row_block) {
-  const int64_t head = blockIdx.x / a.rows;
-  const int row = blockIdx.x % a.rows, rb = row / row_block, r = row % row_block;
-  const int b = (int)(head / a.c.heads), h = (int)(head % a.c.heads);
-  const int pages = pages_of(a, b), lanes = a.c.heads * a.blocks, per = a.plan[1];
-  const int64_t first = a.plan[kPlanHead + b];
-  const bool even = a.plan[0] != 0;
+// The parts of segment (head, row block rb) of sequence b: how many, and part i's slot.
+struct Parts {
   int n;
-  int64_t slot0, step, u0 = 0;
-  if (even) {
-    u0 = first * lanes + (int64_t)(h * a.blocks + rb) * pages;
-    n = pages == 0 ? 0 : (int)((u0 + pages - 1) / per - u0 / per + 1);
-    slot0 = u0 / per * 2;
-    step = 2;
+  int64_t slot0, step;
+  bool even;
+  __device__ __forceinline__ int64_t slot(int i) const { return even && i > 0 ? (slot0 & ~(int64_t)1) + i * step : slot0 + i * step; }
+};
+__device__ __forceinline__ Parts parts_of(const DecodeArgs& a, int b, int h, int rb) {
+  Parts x;
+  const int pages = pages_of(a, b), lanes = a.c.heads * a.blocks, first = a.plan[kPlanHead + b];
+  x.even = a.even;
+  if (a.even) {
+    const int per = a.plan[0], x0 = first * lanes + (h * a.blocks + rb) * (pages + kOpening), u0 = (x0 + kOpening) / per;
+    x.n = pages == 0 ? 0 : (x0 + kOpening + pages - 1) / per - u0 + 1;
+    // the first part is its warp's second piece unless the warp's range begins in the segment
+    x.slot0 = 2 * (int64_t)u0 + (u0 * per < x0 ? 1 : 0);
+    x.step = 2;
   } else {
-    n = (int)(a.plan[kPlanHead + b + 1] - first);
-    slot0 = first * lanes + (int64_t)h * n * a.blocks + rb;
-    step = a.blocks;
+    x.n = a.plan[kPlanHead + b + 1] - first;
+    x.slot0 = (int64_t)first * lanes + (int64_t)h * x.n * a.blocks + rb;
+    x.step = a.blocks;
   }
-  if (n <= 1) return;
-  // in an even cut the first part is its CTA's second piece unless it begins where the CTA does
-  const auto slot = [&](int i) { return slot0 + i * step + (even && i == 0 && u0 % per != 0 ? 1 : 0); };
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  __shared__ float sm[kWarps][2];
-  __shared__ float4 sm_o[kWarps][D / 4];
+  return x;
+}
+
+// The parts of a row together: a warp for each query row of a KV head after an even cut (a few parts each), a CTA where few segments were cut for all
+// CTAs.  Rows of segments that were not cut have nothing to do.
+template <int D, int W>
+__global__ void __launch_bounds__(kThreads) merge_kernel(const DecodeArgs a, int row_block) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = W == 1 ? 0 : tid >> 5;
+  const int64_t all = (int64_t)blockIdx.x * (kWarps / W) + (W == 1 ? tid >> 5 : 0);
+  const int64_t head = all / a.rows;
+  if (head >= (int64_t)a.batch * a.c.heads) return;
+  const int row = (int)(all % a.rows), rb = row / row_block, r = row % row_block;
+  const int b = (int)(head / a.c.heads), h = (int)(head % a.c.heads);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Parts x = parts_of(a, b, h, rb);
+  if (x.n <= 1) return;
+  __shared__ float sm[W][2];
+  __shared__ float4 sm_o[W][D / 4];
   float top = -CUDART_INF_F;
-  for (int i = tid; i < n; i += kThreads) top = fmaxf(top, a.part_ml[(slot(i) * row_block + r) * 2]);
+  for (int i = W == 1 ? lane : tid; i < x.n; i += 32 * W) top = fmaxf(top, a.part_ml[(x.slot(i) * row_block + r) * 2]);
 #pragma unroll
   for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  if (lane == 0) sm[warp][0] = top;
-  __syncthreads();
+  if (W > 1) {
+    if (lane == 0) sm[warp][0] = top;
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w][0]);
+    for (int w = 0; w < W; ++w) top = fmaxf(top, sm[w][0]);
+  }
   const float ref = top == -CUDART_INF_F ? 0.f : top;
   constexpr int kEach = (D / 4 + 31) / 32;
   float4 acc[kEach];
@@ -575,75 +728,131 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const DecodeArgs a, int
   for (int e = 0; e < kEach; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f;
 #pragma unroll 4
-  for (int i = warp; i < n; i += kWarps) {
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (slot(i) * row_block + r) * 2);
+  for (int i = warp; i < x.n; i += W) {
+    const int64_t slot = x.slot(i) * row_block + r;
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + slot * 2);
     const float f = fast_exp2(ml.x - ref);
     sum += ml.y * f;
-    const float4* p = reinterpret_cast<const float4*>(a.part + (slot(i) * row_block + r) * D);
+    const float4* p = reinterpret_cast<const float4*>(a.part + slot * D);
 #pragma unroll
     for (int e = 0; e < kEach; ++e)
       if (lane + e * 32 < D / 4) {
-        const float4 x = p[lane + e * 32];
-        acc[e].x += x.x * f; acc[e].y += x.y * f; acc[e].z += x.z * f; acc[e].w += x.w * f;
+        const float4 v = p[lane + e * 32];
+        acc[e].x += v.x * f; acc[e].y += v.y * f; acc[e].z += v.z * f; acc[e].w += v.w * f;
       }
   }
+  if (W > 1) {
 #pragma unroll
-  for (int e = 0; e < kEach; ++e)
-    if (lane + e * 32 < D / 4) sm_o[warp][lane + e * 32] = acc[e];
-  if (lane == 0) sm[warp][1] = sum;
-  __syncthreads();
-  if (tid < D / 4) {
-    float4 x = sm_o[0][tid];
-    sum = sm[0][1];
+    for (int e = 0; e < kEach; ++e)
+      if (lane + e * 32 < D / 4) sm_o[warp][lane + e * 32] = acc[e];
+    if (lane == 0) sm[warp][1] = sum;
+    __syncthreads();
+    if (warp != 0) return;
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) {
-      const float4 y = sm_o[w][tid];
-      x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+    for (int w = 1; w < W; ++w) {
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+        if (lane + e * 32 < D / 4) {
+          const float4 v = sm_o[w][lane + e * 32];
+          acc[e].x += v.x; acc[e].y += v.y; acc[e].z += v.z; acc[e].w += v.w;
+        }
       sum += sm[w][1];
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    uint2 packed = make_uint2(pack_out16x2(x.x * inv, x.y * inv, a.bf16), pack_out16x2(x.z * inv, x.w * inv, a.bf16));
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (head * a.rows + row) * D + tid * 4) = packed;
-    if (a.lse != nullptr && tid == 0) a.lse[head * a.rows + row] = sum == 0.f ? CUDART_INF_F : ref + log2f(sum);
   }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint16_t* out = static_cast<uint16_t*>(a.out) + (head * a.rows + row) * D;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e)
+    if (lane + e * 32 < D / 4)
+      *reinterpret_cast<uint2*>(out + (lane + e * 32) * 4) =
+          make_uint2(pack_out16x2(acc[e].x * inv, acc[e].y * inv, a.bf16), pack_out16x2(acc[e].z * inv, acc[e].w * inv, a.bf16));
+  if (a.lse != nullptr && lane == 0) a.lse[head * a.rows + row] = sum == 0.f ? CUDART_INF_F : ref + log2f(sum);
 }
 
-// mass_j += sum over rows of 2^(score - log-sum): a thread for each key.
-__global__ void __launch_bounds__(256) mass_kernel(const DecodeArgs a, int row_block) {
-  const int64_t head = blockIdx.y;
-  const int b = (int)(head / a.c.heads), h = (int)(head % a.c.heads);
+// mass_j += sum over rows of 2^(score - log of the row's sum): a CTA for each KV head and 1024 keys, four keys a thread, a row's four scores in one load.
+constexpr int kEachKey = 4, kMassThreads = 256, kMassKeys = kEachKey * kMassThreads;
+__global__ void __launch_bounds__(kMassThreads) mass_kernel(const DecodeArgs a, int row_block, int chunks) {
+  const int64_t head = blockIdx.x / chunks;
+  const int b = (int)(head / a.c.heads), h = (int)(head % a.c.heads), j0 = blockIdx.x % chunks * kMassKeys + threadIdx.x;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int len = min(len_of(a, b), a.mass_cap);
-  const int j = blockIdx.x * 256 + threadIdx.x;
-  if (j >= len) return;
+  if (j0 - (int)threadIdx.x >= len) return;
   const int at = a.mass_index != nullptr ? a.mass_index[b] : b;
   if (at < 0 || at >= a.mass_rows) {
-    if (j == 0) atomicOr(a.c.status, kStatusBadPageId);
+    if (threadIdx.x == 0) atomicOr(a.c.status, kStatusBadPageId);
     return;
   }
-  float sum = 0.f;
+  float* mass = a.mass + ((int64_t)at * a.c.heads + h) * a.mass_cap;
+  float had[kEachKey], got[kEachKey];
+#pragma unroll
+  for (int k = 0; k < kEachKey; ++k) {
+    had[k] = j0 + k * kMassThreads < len ? mass[j0 + k * kMassThreads] : 0.f;
+    got[k] = 0.f;
+  }
   for (int rb = 0; rb < a.blocks; ++rb) {
-    const float* s = a.scores + (((head * a.blocks + rb) * a.c.max_pages) * kPage + j) * a.score_cols;
+    const float* s = a.scores + ((head * a.blocks + rb) * a.c.max_pages * kPage + j0) * a.score_cols;
     const float* lse = a.lse + head * a.rows + rb * row_block;
     const int rows = min(row_block, a.rows - rb * row_block);
-    for (int r = 0; r < rows; ++r) sum += fast_exp2(s[r] - lse[r]);
+    if (a.score_cols % 4 == 0) {
+      for (int r = 0; r < rows; r += 4) {
+        float4 v[kEachKey];
+#pragma unroll
+        for (int k = 0; k < kEachKey; ++k)
+          if (j0 + k * kMassThreads < len) v[k] = __ldcs(reinterpret_cast<const float4*>(s + (int64_t)k * kMassThreads * a.score_cols + r));
+        float n[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) n[e] = r + e < rows ? lse[r + e] : CUDART_INF_F;
+#pragma unroll
+        for (int k = 0; k < kEachKey; ++k)
+          if (j0 + k * kMassThreads < len) {
+            const float w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (r + e < rows) got[k] += fast_exp2(w[e] - n[e]);
+          }
+      }
+    } else {
+      for (int r = 0; r < rows; ++r)
+#pragma unroll
+        for (int k = 0; k < kEachKey; ++k)
+          if (j0 + k * kMassThreads < len) got[k] += fast_exp2(s[(int64_t)k * kMassThreads * a.score_cols + r] - lse[r]);
+    }
   }
-  a.mass[((int64_t)at * a.c.heads + h) * a.mass_cap + j] += sum;
+#pragma unroll
+  for (int k = 0; k < kEachKey; ++k)
+    if (j0 + k * kMassThreads < len) mass[j0 + k * kMassThreads] = had[k] + got[k];
+}
+
+// Behind the kernel before it in the stream: its blocks come as soon as there is room, and wait for that kernel's end before they read.
+template <class... Params, class... Args>
+cudaError_t launch_behind(void (*kernel)(Params...), int64_t grid, int threads, size_t smem, cudaStream_t s, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 template <int D, int NT, bool E4M3>
 cudaError_t launch_decode_as(const DecodeArgs& a, cudaStream_t s) {
   constexpr int kRows = NT * 8;
-  const size_t smem = (((size_t)a.batch + 1 + 3) & ~(size_t)3) * 4 + (size_t)kWarps * kRows * (D + 6) * 4;
+  const size_t smem = (size_t)kWarps * Shape<D, NT>::kWarpBytes + ((size_t)2 * a.batch + 1) * 4;
   static SharedMemoryLimit limit;
   cudaError_t e = limit.raise(reinterpret_cast<const void*>(decode_kernel<D, NT, E4M3>), (int)smem);
   if (e != cudaSuccess) return e;
-  decode_kernel<D, NT, E4M3><<<a.n_cta, kThreads, smem, s>>>(a);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  merge_kernel<D><<<(unsigned)((int64_t)a.batch * a.c.heads * a.rows), kThreads, 0, s>>>(a, kRows);
-  if ((e = cudaGetLastError()) != cudaSuccess || a.mass == nullptr) return e;
-  const dim3 grid((unsigned)(((int64_t)a.c.max_pages * kPage + 255) / 256), (unsigned)(a.batch * a.c.heads));
-  mass_kernel<<<grid, 256, 0, s>>>(a, kRows);
-  return cudaGetLastError();
+  if ((e = launch_behind(decode_kernel<D, NT, E4M3>, a.n_cta, kThreads, smem, s, a)) != cudaSuccess) return e;
+  const int64_t rows = (int64_t)a.batch * a.c.heads * a.rows;
+  if (a.even) e = launch_behind(merge_kernel<D, 1>, (rows + kWarps - 1) / kWarps, kThreads, 0, s, a, kRows);
+  else if (a.c.max_pages > kLeastPart) e = launch_behind(merge_kernel<D, kWarps>, rows, kThreads, 0, s, a, kRows);      // (else no segment is cut)
+  if (e != cudaSuccess || a.mass == nullptr) return e;
+  const int chunks = (int)(((int64_t)a.c.max_pages * kPage + kMassKeys - 1) / kMassKeys);
+  return launch_behind(mass_kernel, (int64_t)chunks * a.batch * a.c.heads, kMassThreads, 0, s, a, kRows, chunks);
 }
 
 template <int D, int NT>
@@ -652,7 +861,7 @@ cudaError_t launch_decode_codes(const DecodeArgs& a, bool e4m3, cudaStream_t s) 
 }
 
 template <int D, int NT>
-constexpr int ctas_of() { return Shape<D, NT, false>::kCtas; }
+constexpr int ctas_of() { return Shape<D, NT>::kCtas; }
 
 }  // namespace
 
@@ -663,12 +872,13 @@ DecodeShape decode_shape(int dim, int rows, int sms) {
   d.blocks = (rows + d.row_block - 1) / d.row_block;
   const int ctas = dim == 64 ? (wide ? ctas_of<64, 2>() : ctas_of<64, 1>()) : dim == 128 ? (wide ? ctas_of<128, 2>() : ctas_of<128, 1>()) : ctas_of<256, 1>();
   d.n_cta = sms * ctas;
-  d.slots = 2 * d.n_cta;
+  d.slots = 2 * d.n_cta * kWarps;
   d.score_cols = rows >= d.row_block ? d.row_block : (rows + 1) & ~1;
   return d;
 }
 
 cudaError_t launch_decode(DecodeArgs a, bool e4m3, cudaStream_t s) {
+  a.even = 2 * (int64_t)a.batch * a.c.heads * a.blocks > a.n_cta;
   const bool wide = a.rows > 8 && a.c.dim <= 128;
   switch (a.c.dim) {
     case 64: return wide ? launch_decode_codes<64, 2>(a, e4m3, s) : launch_decode_codes<64, 1>(a, e4m3, s);
