@@ -356,6 +356,23 @@ def test_evict_long_sequences(fa, lens, budget):
     _evict_case(fa, torch.int8, 2, 64, lens, budget, min(4, budget), 0, 85)
 
 
+def test_evict_behind_a_table_of_very_many_pages(fa):
+    """A table whose rows could hold more tokens than the clusters' shared memory has keys."""
+    g = torch.Generator().manual_seed(91)
+    lens, width = [3000, 700, 4100], 20600
+    table, rest = kc.tables(lens, 520, 92, width=width)
+    new = _ints([rest[b * 4: b * 4 + 4] for b in range(3)])
+    state = kc.cache(520, 1, 64, torch.int8, 93)
+    mass = torch.zeros(3, 1, width * 16)
+    mass[:, :, :4200] = torch.randint(0, 50, (3, 1, 4200), generator=g).float()
+    dev, ref = [t.cuda() for t in state], [t.clone() for t in state]
+    got = fa.evict_paged_kv8(mass.cuda(), *dev, table.cuda(), _ints(lens).cuda(), width, new.cuda(), 60, 1, 9)
+    want = orc.evict(mass, *ref, table, lens, new, 60, 1, 9)
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
+    for a, b in zip(dev, ref):
+        _same(a, b)
+
+
 def test_evict_rows_of_sums_by_index(fa):
     g = torch.Generator().manual_seed(86)
     _evict_case(fa, torch.int8, 2, 64, [100, 60, 80], 40, 1, 5, 87, torch.rand(7, 2, 128, generator=g), _ints([5, 0, 3]))
