@@ -143,6 +143,7 @@ _k8 = _c.POINTER(Kv8Cache)
 KV8_SIGNATURES = {
     "fak_last_error": (_c.c_char_p, []),
     "fak_status": (_i, [_vp, _c.POINTER(_i), _i]),
+    "fak_devices": (_c.c_uint64, []),
     "fak_append_paged": (_i, [_k8, _vp, _vp, _i64, _i64, _i, _vp, _vp, _i, _i64, _vp]),
     "fak_decode_workspace": (_sz, [_k8, _i, _i, _i, _i]),
     "fak_decode_paged": (_i, [_k8, _vp, _vp, _vp, _i, _i, _i, _i, _f, _vp, _vp, _i, _i, _vp, _sz, _vp]),
@@ -203,3 +204,9 @@ def call_module(workspaces):
     entries = [n for n in SIGNATURES if n.startswith(("fa_last", "fa_decode", "fa_paged", "fa_prefill"))]
     module.bind({n: _c.cast(getattr(lib, n), _vp).value for n in entries}, workspaces)
     return module
+
+
+def bind_kv8(module) -> None:
+    """The operators on the 8-bit cache through that module, too."""
+    lib = library("kv8")
+    module.bind_kv8({n: _c.cast(getattr(lib, n), _vp).value for n in KV8_SIGNATURES})

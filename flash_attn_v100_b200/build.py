@@ -147,7 +147,7 @@ def call_fits(path: str) -> bool:
 
 def build_call(force: bool = False) -> str:
     """Compile the host side of the calls.  The operators work without it, through ctypes, at a higher cost per call."""
-    deps = (CALL_SOURCE, os.path.join(INCLUDE, "fa_b200.h"))
+    deps = (CALL_SOURCE, os.path.join(INCLUDE, "fa_b200.h"), os.path.join(INCLUDE, "fa_b200_kv8.h"))
     if not force and call_fits(CALL_PATH) and os.path.getmtime(CALL_PATH) >= max(os.path.getmtime(d) for d in deps):
         return CALL_PATH
     import torch

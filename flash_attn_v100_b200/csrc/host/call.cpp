@@ -20,6 +20,7 @@
 #include <climits>
 
 #include "../../../include/fa_b200.h"
+#include "../../../include/fa_b200_kv8.h"
 
 namespace {
 
@@ -36,6 +37,14 @@ struct Entries {
   decltype(&fa_prefill_varlen_zeroed) varlen;
 };
 Entries g;
+struct Kv8Entries {
+  decltype(&fak_last_error) last_error;
+  decltype(&fak_append_paged) append;
+  decltype(&fak_decode_workspace) workspace;
+  decltype(&fak_decode_paged) decode;
+  decltype(&fak_evict_paged) evict;
+};
+Kv8Entries g8{};
 PyObject* g_workspaces = nullptr;      // ops._workspaces: (device, stream) -> uint8 tensor
 
 // Arguments of a call, looked at once.  `ok` turns false where the call is not the plain case.
@@ -309,19 +318,187 @@ PyObject* varlen(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- the paged 8-bit cache (kv8_ops.py) ----
+PyObject* kv8_failed() {
+  const char* why = g8.last_error();
+  PyErr_SetString(PyExc_RuntimeError, why != nullptr && why[0] != 0 ? why : "a call of the kv8 library failed");
+  return nullptr;
+}
+bool of_type(Call& c, PyObject* o, at::ScalarType a, at::ScalarType b, at::ScalarType* type) {
+  if (!c.ok || !THPVariable_CheckExact(o)) return false;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.defined()) return false;
+  *type = t.scalar_type();
+  return *type == a || *type == b;
+}
+// a[0 .. 3]: k_cache, v_cache, kv_scale, block_table; its row stride; a sequence for each of `batch`.
+bool kv8_cache(Call& c, PyObject* const* a, int width, int64_t batch, FakCache* cache) {
+  at::ScalarType codes;
+  if (!of_type(c, a[0], at::kChar, at::kFloat8_e4m3fn, &codes)) return false;
+  const at::Tensor *k = c.tensor(a[0], codes, 4), *v = c.tensor(a[1], codes, 4), *scale = c.tensor(a[2], at::kFloat, 3), *table = c.tensor(a[3], at::kInt, 2);
+  if (!c.ok) return false;
+  const int64_t pages = k->size(0), heads = k->size(1), dim = k->size(3), used = std::min<int64_t>(width, table->size(1));
+  c.need(k->sizes() == v->sizes() && k->size(2) == 16 && (dim == 64 || dim == 128 || dim == 256) && pages > 0 && pages <= INT_MAX && heads > 0 && heads < 32768);
+  c.need(scale->size(0) == pages && scale->size(1) == heads && scale->size(2) == 2);
+  c.need(batch > 0 && batch <= (1 << 24) && table->size(0) >= batch && used > 0 && (batch - 1) * width + used <= table->numel());
+  if (!c.ok) return false;
+  *cache = {k->data_ptr(), v->data_ptr(), scale->data_ptr<float>(), pages, (int32_t)heads, (int32_t)dim, codes == at::kChar ? FAK_INT8 : FAK_E4M3,
+            table->data_ptr<int32_t>(), width, (int32_t)used};
+  return true;
+}
+const at::Tensor* kv8_ints(Call& c, PyObject* o, int64_t n) {
+  const at::Tensor* t = c.tensor(o, at::kInt, 1);
+  if (t != nullptr) c.need(t->numel() == n);
+  return t;
+}
+// mass and mass_index (either may be None)
+struct Kv8Mass {
+  const at::Tensor *mass = nullptr, *index = nullptr;
+  Kv8Mass(Call& c, PyObject* m, PyObject* i, const FakCache& cache, int64_t batch) {
+    if (m != Py_None) mass = c.tensor(m, at::kFloat, 3);
+    if (i != Py_None) index = kv8_ints(c, i, batch);
+    if (!c.ok) return;
+    c.need(mass != nullptr || index == nullptr);
+    if (mass != nullptr)
+      c.need(mass->size(1) == cache.heads && mass->size(2) >= (int64_t)cache.max_pages * 16 && mass->size(2) <= INT_MAX && mass->size(0) <= INT_MAX &&
+             mass->size(0) >= (index != nullptr ? 1 : batch));
+  }
+  float* data() const { return mass != nullptr ? mass->data_ptr<float>() : nullptr; }
+  const int32_t* at() const { return index != nullptr ? index->data_ptr<int32_t>() : nullptr; }
+  int rows() const { return mass != nullptr ? (int)mass->size(0) : 0; }
+  int cap() const { return mass != nullptr ? (int)mass->size(2) : 0; }
+};
+
+// (k, v, k_cache, v_cache, kv_scale, block_table, positions, max_num_blocks, cu_seqlens) -> True
+PyObject* kv8_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Call c(n == 9 && g8.append != nullptr);
+  at::ScalarType type;
+  if (!c.ok || !of_type(c, a[0], at::kHalf, at::kBFloat16, &type)) Py_RETURN_NONE;
+  const bool packed = a[8] != Py_None;
+  const at::Tensor *k = c.tensor(a[0], type, packed ? 3 : 4), *v = c.tensor(a[1], type, packed ? 3 : 4), *cu = nullptr, *positions = nullptr;
+  if (packed) cu = c.tensor(a[8], at::kInt, 1);
+  const int width = c.integer(a[7]);
+  if (!c.ok) Py_RETURN_NONE;
+  const int64_t total = k->size(0), batch = packed ? cu->numel() - 1 : total;
+  if (a[6] != Py_None) positions = kv8_ints(c, a[6], batch);
+  FakCache cache;
+  if (!c.ok || !kv8_cache(c, a + 2, width, batch, &cache)) Py_RETURN_NONE;
+  c.need(k->sizes() == v->sizes() && k->size(1) == cache.heads && k->size(packed ? 2 : 3) == cache.dim && (packed || (k->size(2) == 1 && positions != nullptr)) && total > 0 &&
+         (reinterpret_cast<uintptr_t>(k->data_ptr()) | reinterpret_cast<uintptr_t>(v->data_ptr())) % 16 == 0);
+  if (!c.ok) Py_RETURN_NONE;
+  const int64_t stride = (int64_t)cache.heads * cache.dim;
+  const cudaStream_t s = stream_of(c.dev);
+  int rc;
+  FA_LAUNCH(g8.append(&cache, k->data_ptr(), v->data_ptr(), stride, stride, type == at::kBFloat16 ? FAK_BF16 : FAK_F16,
+                      positions != nullptr ? positions->data_ptr<int32_t>() : nullptr, packed ? cu->data_ptr<int32_t>() : nullptr, (int)batch, total, s));
+  if (rc != 0) return kv8_failed();
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, k_cache, v_cache, kv_scale, block_table, seq_lens, max_num_blocks, softcap, mass, mass_index)
+PyObject* kv8_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Call c(n == 10 && g8.decode != nullptr);
+  at::ScalarType type;
+  if (!c.ok || !PyFloat_CheckExact(a[7]) || !of_type(c, a[0], at::kHalf, at::kBFloat16, &type)) Py_RETURN_NONE;
+  const double softcap = PyFloat_AS_DOUBLE(a[7]);
+  const at::Tensor* q = c.tensor(a[0], type, 4);
+  const int width = c.integer(a[6]);
+  c.need(softcap >= 0.0 && softcap <= 1e30);
+  if (!c.ok) Py_RETURN_NONE;
+  const int64_t batch = q->size(0), heads = q->size(1), tokens = q->size(2);
+  FakCache cache;
+  if (!kv8_cache(c, a + 1, width, batch, &cache)) Py_RETURN_NONE;
+  const at::Tensor* lens = kv8_ints(c, a[5], batch);
+  const Kv8Mass mass(c, a[8], a[9], cache, batch);
+  c.need(q->size(3) == cache.dim && heads <= (1 << 20) && tokens > 0 && tokens <= 65536);
+  c.heads(heads, cache.heads);
+  if (!c.ok) Py_RETURN_NONE;
+  const size_t bytes = g8.workspace(&cache, (int)batch, (int)heads, (int)tokens, mass.mass != nullptr);
+  const at::Tensor out = at::empty(q->sizes(), q->options()), ws = at::empty({(int64_t)bytes}, q->options().dtype(at::kByte));
+  const cudaStream_t s = stream_of(c.dev);
+  int rc;
+  FA_LAUNCH(g8.decode(&cache, q->data_ptr(), out.data_ptr(), lens->data_ptr<int32_t>(), (int)batch, (int)heads, (int)tokens,
+                      type == at::kBFloat16 ? FAK_BF16 : FAK_F16, (float)softcap, mass.data(), mass.at(), mass.rows(), mass.cap(), ws.data_ptr(), bytes, s));
+  if (rc != 0) return kv8_failed();
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// (mass, k_cache, v_cache, kv_scale, block_table, seq_lens, max_num_blocks, new_block_table, budget, sink, recent, mass_index) -> (kept, new_lens, new_mass)
+PyObject* kv8_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Call c(n == 12 && g8.evict != nullptr);
+  const int width = c.ok ? c.integer(a[6]) : 0, budget = c.ok ? c.integer(a[8]) : 0, sink = c.ok ? c.integer(a[9]) : 0, recent = c.ok ? c.integer(a[10]) : 0;
+  const at::Tensor *lens = c.ok ? c.tensor(a[5], at::kInt, 1) : nullptr, *fresh = c.ok ? c.tensor(a[7], at::kInt, 2) : nullptr;
+  if (!c.ok) Py_RETURN_NONE;
+  const int64_t batch = lens->numel();
+  FakCache cache;
+  if (!kv8_cache(c, a + 1, width, batch, &cache)) Py_RETURN_NONE;
+  const Kv8Mass mass(c, a[0], a[11], cache, batch);
+  c.need(mass.mass != nullptr && budget > 0 && sink >= 0 && recent >= 0 && (int64_t)sink + recent <= budget && fresh->size(0) >= batch &&
+         fresh->size(1) * 16 >= budget && fresh->size(1) <= INT_MAX);
+  if (!c.ok) Py_RETURN_NONE;
+  const at::Tensor kept = at::empty({batch, cache.heads, budget}, lens->options()), new_lens = at::empty({batch}, lens->options()),
+                   new_mass = at::empty({batch, cache.heads, budget}, mass.mass->options());
+  const cudaStream_t s = stream_of(c.dev);
+  int rc;
+  FA_LAUNCH(g8.evict(&cache, mass.data(), mass.at(), mass.rows(), mass.cap(), lens->data_ptr<int32_t>(), (int)batch, fresh->data_ptr<int32_t>(),
+                     (int)fresh->size(1), budget, sink, recent, kept.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(), new_mass.data_ptr<float>(), s));
+  if (rc != 0) return kv8_failed();
+  PyObject* r = PyTuple_New(3);
+  if (r == nullptr) return nullptr;
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(kept));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(new_lens));
+  PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(new_mass));
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// Entry points from a dictionary of addresses by name.
+struct Lookup {
+  PyObject* names;
+  bool ok = true;
+  template <class F>
+  void operator()(const char* name, F& fn) {
+    PyObject* v = PyDict_GetItemString(names, name);
+    void* p = v != nullptr ? PyLong_AsVoidPtr(v) : nullptr;
+    ok = ok && p != nullptr;
+    fn = reinterpret_cast<F>(p);
+  }
+  PyObject* missing() const {
+    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "an entry point is missing");
+    return nullptr;
+  }
+};
+
+// bind_kv8(entry addresses by name)
+PyObject* bind_kv8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 1 || !PyDict_Check(a[0])) {
+    PyErr_SetString(PyExc_TypeError, "bind_kv8 takes a dictionary");
+    return nullptr;
+  }
+  Lookup get{a[0]};
+  Kv8Entries e{};
+  get("fak_last_error", e.last_error);
+  get("fak_append_paged", e.append);
+  get("fak_decode_workspace", e.workspace);
+  get("fak_decode_paged", e.decode);
+  get("fak_evict_paged", e.evict);
+  if (!get.ok) return get.missing();
+  g8 = e;
+  Py_RETURN_NONE;
+}
+
 // bind(entry addresses by name, ops._workspaces)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 2 || !PyDict_Check(a[0]) || !PyDict_Check(a[1])) {
     PyErr_SetString(PyExc_TypeError, "bind takes two dictionaries");
     return nullptr;
   }
-  bool ok = true;
-  auto get = [&](const char* name, auto& fn) {
-    PyObject* v = PyDict_GetItemString(a[0], name);
-    void* p = v != nullptr ? PyLong_AsVoidPtr(v) : nullptr;
-    ok = ok && p != nullptr;
-    fn = reinterpret_cast<std::remove_reference_t<decltype(fn)>>(p);
-  };
+  Lookup get{a[0]};
   get("fa_last_error", g.last_error);
   get("fa_decode_workspace_bytes", g.workspace_bytes);
   get("fa_paged_decode_gqa_f16", g.paged);
@@ -336,10 +513,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   get("fa_prefill_dense_f16", g.dense);
   get("fa_prefill_dense_bf16", g.dense_bf16);
   get("fa_prefill_varlen_zeroed", g.varlen);
-  if (!ok) {
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "an entry point is missing");
-    return nullptr;
-  }
+  if (!get.ok) return get.missing();
   Py_INCREF(a[1]);
   Py_XSETREF(g_workspaces, a[1]);
   Py_RETURN_NONE;
@@ -347,7 +521,8 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #define FA_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {FA_METHOD(bind),   FA_METHOD(paged),   FA_METHOD(decode), FA_METHOD(contig), FA_METHOD(window),
-                           FA_METHOD(int8_kv), FA_METHOD(int8_qk), FA_METHOD(dense),  FA_METHOD(varlen), {nullptr, nullptr, 0, nullptr}};
+                           FA_METHOD(int8_kv), FA_METHOD(int8_qk), FA_METHOD(dense),  FA_METHOD(varlen), FA_METHOD(bind_kv8), FA_METHOD(kv8_append),
+                           FA_METHOD(kv8_decode), FA_METHOD(kv8_evict), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_call", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -14,6 +14,8 @@ namespace k8 = fa::kv8;
 
 __device__ int g_status;      // of a device: every launch on it shares the word, which needs no allocation and no clearing before a capture
 
+std::atomic<uint64_t> g_devices;
+
 cudaError_t status_word(int** word) {
   static std::atomic<int*> cached[64];
   int dev = 0;
@@ -23,7 +25,10 @@ cudaError_t status_word(int** word) {
   void* p = nullptr;
   if ((e = cudaGetSymbolAddress(&p, g_status)) != cudaSuccess) return e;
   *word = static_cast<int*>(p);
-  if (dev >= 0 && dev < 64) cached[dev].store(*word, std::memory_order_release);
+  if (dev >= 0 && dev < 64) {
+    cached[dev].store(*word, std::memory_order_release);
+    g_devices.fetch_or(1ull << dev);
+  }
   return cudaSuccess;
 }
 
@@ -98,6 +103,8 @@ int fak_status(void* stream, int* status, int clear) {
   if (*status != 0) return fail(FAK_ERR_DEVICE_STATUS, "a kernel on the 8-bit cache met a page or a row of sums outside the cache (status %d)", *status);
   return FAK_OK;
 }
+
+uint64_t fak_devices(void) { return g_devices.load(); }
 
 int fak_append_paged(const FakCache* cache, const void* k, const void* v, int64_t k_stride, int64_t v_stride, int dtype, const int32_t* positions,
                      const int32_t* cu_seqlens, int batch, int64_t total, void* stream) {

@@ -13,15 +13,27 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import PAGE_BLOCK_SIZE, SUPPORTED_D, _check_dim, _check_gqa_heads, _check_input, _chk, _on, _ptr, _same_device, _stream_ptr
+from .ops import (PAGE_BLOCK_SIZE, SUPPORTED_D, _check_dim, _check_gqa_heads, _check_input, _chk, _native_module, _on, _ptr, _same_device, _stream_ptr,
+                  _UNSET)
 
 _ROWS = {torch.float16: 0, torch.bfloat16: 1}
 _CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
-_used = set()      # devices whose status word a kernel may have written
+_call_mod = _UNSET
 
 
 def _kv8():
     return _lib.library("kv8")
+
+
+def _native(name, *args):
+    """The call `name` of the native host side (csrc/host/call.cpp); None where the call is anything but the plain case, which the wrappers below then look at."""
+    global _call_mod
+    if _call_mod is _UNSET:
+        module = _native_module()
+        if module is not None:
+            _lib.bind_kv8(module)
+        _call_mod = module
+    return None if _call_mod is None else getattr(_call_mod, name)(*args)
 
 
 def _rc(rc):
@@ -48,7 +60,6 @@ def _cache(k_cache, v_cache, kv_scale, block_table, batch, max_num_blocks):
     _chk(max_num_blocks > 0, "max_num_blocks must be positive")
     used = min(max_num_blocks, block_table.size(1))
     _chk(used > 0 and (batch - 1) * max_num_blocks + used <= block_table.numel(), "max_num_blocks (row stride) is larger than block_table allows")
-    _used.add(k_cache.get_device())
     return _lib.Kv8Cache(k=_ptr(k_cache), v=_ptr(v_cache), scale=_ptr(kv_scale), pages=pages, heads=heads, dim=dim, codes=_CODES[k_cache.dtype],
                          table=_ptr(block_table), width=max_num_blocks, max_pages=used)
 
@@ -75,6 +86,8 @@ def append_paged_kv8(k, v, k_cache, v_cache, kv_scale, block_table, positions, m
     multiple of 8 elements apart (slices of a fused projection).  Per page, head and kind: the scale is the largest magnitude of its rows / 127
     (e4m3: 448), at least 2^-100.  Where a page goes on being filled its scale only grows, and the codes it has are then rounded again.  NaN and
     infinities make a page's scale infinite, and what attends to it NaN.  Two sequences of a call must not write to the same page."""
+    if _native("kv8_append", k, v, k_cache, v_cache, kv_scale, block_table, positions, max_num_blocks, cu_seqlens):
+        return
     _chk(isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor), "k and v must be tensors")
     _chk(k.is_cuda and v.is_cuda, "k and v must be CUDA tensors")
     _chk(k.dtype in _ROWS, "k must be float16 or bfloat16")
@@ -124,6 +137,9 @@ def forward_paged_decode_gqa_kv8(q, k_cache, v_cache, kv_scale, block_table, seq
     sees none gets zeros.  With softcap > 0 a score x becomes softcap * tanh(x / softcap).  `mass` [rows,H_KV,tokens] fp32: what every key
     is given by the softmax, summed over the query heads of its KV head and the T tokens, is added in place to row mass_index[b] (None: b); the
     rows of a call must be different ones."""
+    done = _native("kv8_decode", q, k_cache, v_cache, kv_scale, block_table, seq_lens, max_num_blocks, softcap, mass, mass_index)
+    if done is not None:
+        return done
     _check_input(q, "q")
     _check_dim(q, 4, "q")
     _chk(q.dtype in _ROWS, "q must be float16 or bfloat16")
@@ -160,6 +176,9 @@ def evict_paged_kv8(mass, k_cache, v_cache, kv_scale, block_table, seq_lens, max
     int32, which must be none of the pages that block_table's rows hold: those are left as they were.  A new page's scale is the largest of its tokens', and
     codes from a smaller one are rounded again.  mass as in `forward_paged_decode_gqa_kv8`.  Returns (indices kept [B,H_KV,budget] int32, -1 behind
     the last; new seq_lens [B] int32; their mass [B,H_KV,budget] fp32, 0 behind the last)."""
+    done = _native("kv8_evict", mass, k_cache, v_cache, kv_scale, block_table, seq_lens, max_num_blocks, new_block_table, budget, sink, recent, mass_index)
+    if done is not None:
+        return done
     _chk(isinstance(seq_lens, torch.Tensor) and seq_lens.dim() == 1, "seq_lens must be a 1D tensor")
     batch = seq_lens.numel()
     c = _cache(k_cache, v_cache, kv_scale, block_table, batch, max_num_blocks)
@@ -185,8 +204,11 @@ def evict_paged_kv8(mass, k_cache, v_cache, kv_scale, block_table, seq_lens, max
 
 def check_errors(device=None) -> None:
     """Synchronise and raise RuntimeError if an operator on an 8-bit cache has met a page outside it since the last check."""
-    for dev in sorted(_used):
-        if device is not None and torch.device(device).index not in (None, dev):
+    if "kv8" not in _lib._libs:
+        return
+    used = _kv8().fak_devices()
+    for dev in range(used.bit_length()):
+        if not used >> dev & 1 or device is not None and torch.device(device).index not in (None, dev):
             continue
         with torch.cuda.device(dev):
             st = ctypes.c_int(0)

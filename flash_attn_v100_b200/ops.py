@@ -73,11 +73,17 @@ _UNSET = object()
 _call_mod = _UNSET
 
 
-def _native(name, *args):
-    """The call `name` of the native host side with these arguments; None if it is not for it (or not there)."""
+def _native_module():
     global _call_mod
     if _call_mod is _UNSET:
         _call_mod = _lib.call_module(_workspaces)
+    return _call_mod
+
+
+def _native(name, *args):
+    """The call `name` of the native host side with these arguments; None if it is not for it (or not there)."""
+    if _call_mod is _UNSET:
+        _native_module()
     return None if _call_mod is None else getattr(_call_mod, name)(*args)
 
 

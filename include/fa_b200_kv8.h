@@ -35,6 +35,8 @@ const char* fak_last_error(void);
 /* Waits for `stream` and reads the status word of the current device: FAK_ERR_DEVICE_STATUS if a page outside the cache was met (bit 1 of
  * *status) since it was last cleared. */
 int fak_status(void* stream, int* status, int clear);
+/* Devices (bit i: device i) that an operator has been called on. */
+uint64_t fak_devices(void);
 
 /* New rows into pages.  k, v: `total` tokens of [heads, dim], k_stride and v_stride elements from token to token (multiples of 8).  Sequence b has the
  * tokens cu_seqlens[b] to cu_seqlens[b + 1] (null: token b alone, total == batch) and puts them at positions[b] and on (null: 0).

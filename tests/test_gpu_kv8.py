@@ -567,3 +567,85 @@ def test_cache_class_serves_and_evicts(fa):
     assert c.evict(["a", "b"], 100) == 0
     c.release("a"); c.release("b")
     assert c.get_num_free_blocks() == 64
+
+
+# ---- the host side -------------------------------------------------------------------------------------------------
+def test_native_host_side_and_python_do_the_same(fa, monkeypatch):
+    from flash_attn_v100_b200 import kv8_ops
+    H, D, lens = 2, 64, [70, 20]
+    table, rest = kc.tables(lens, 16, 110)
+    g = torch.Generator().manual_seed(111)
+    k, v, q = (torch.randn(2, n, 1, D, generator=g).half().cuda() for n in (H, H, 4 * H))
+    kp, vp = (torch.randn(25, H, D, generator=g).half().cuda() for _ in range(2))
+    new, mass0 = _ints([rest[:2], rest[2:4]]).cuda(), torch.rand(3, H, table.size(1) * 16, generator=g).cuda()
+    index, n = _ints([2, 0]).cuda(), _ints(lens).cuda()
+
+    def run():
+        dev = [t.cuda() for t in kc.cache(16, H, D, torch.float8_e4m3fn, 112)]
+        bt, mass = table.cuda(), mass0.clone()
+        fa.append_paged_kv8(kp, vp, *dev, bt, _ints([3, 0]).cuda(), bt.size(1), cu_seqlens=_ints([0, 20, 25]).cuda())
+        fa.append_paged_kv8(k, v, *dev, bt, n - 1, bt.size(1))
+        outs = [fa.forward_paged_decode_gqa_kv8(q, *dev, bt, n, bt.size(1)),
+                fa.forward_paged_decode_gqa_kv8(q, *dev, bt, n, bt.size(1), softcap=7.0, mass=mass, mass_index=index)]
+        outs += fa.evict_paged_kv8(mass, *dev, bt, n, bt.size(1), new, 30, 2, 4, mass_index=index)
+        return [t.cpu() for t in outs + dev + [mass]]
+
+    calls = []
+    module = kv8_ops._native_module()
+    assert module is not None
+    native = kv8_ops._native
+    monkeypatch.setattr(kv8_ops, "_native", lambda name, *a: calls.append((name, native(name, *a))) or calls[-1][1])
+    fast = run()
+    assert [name for name, _ in calls] == ["kv8_append", "kv8_append", "kv8_decode", "kv8_decode", "kv8_evict"] and all(r is not None for _, r in calls)
+    monkeypatch.setattr(kv8_ops, "_native", lambda name, *a: None)
+    slow = run()
+    for a, b in zip(fast, slow):
+        assert torch.equal(kc.bits(a), kc.bits(b))
+
+
+def test_calls_that_do_not_fit_are_refused(fa):
+    H, D = 2, 64
+    k8, v8, scale = (t.cuda() for t in kc.cache(4, H, D, torch.int8, 113))
+    table, n = _ints([[0, 1]]).cuda(), _ints([20]).cuda()
+    q, k = torch.zeros(1, 4, 1, D).half().cuda(), torch.zeros(1, H, 1, D).half().cuda()
+    mass, new = torch.zeros(1, H, 32).cuda(), _ints([[2, 3]]).cuda()
+    decode = lambda q=q, k8=k8, v8=v8, scale=scale, table=table, n=n, width=2, **kw: fa.forward_paged_decode_gqa_kv8(q, k8, v8, scale, table, n, width, **kw)
+    append = lambda k=k, v=k, n=n, **kw: fa.append_paged_kv8(k, v, k8, v8, scale, table, n, 2, **kw)
+    evict = lambda mass=mass, new=new, budget=16, **kw: fa.evict_paged_kv8(mass, k8, v8, scale, table, n, 2, new, budget, **kw)
+    for call, message in (
+            (lambda: decode(q=q.float()), "q must be float16 or bfloat16"),
+            (lambda: decode(q=q.transpose(1, 3)), "contiguous"),
+            (lambda: decode(q=q[:, :3].contiguous()), "divisible"),
+            (lambda: decode(q=torch.zeros(1, 4, 0, D).half().cuda()), "at least one token"),
+            (lambda: decode(q=torch.zeros(2, 4, 1, D).half().cuda()), "block_table batch size"),
+            (lambda: decode(q=torch.zeros(1, 4, 1, 128).half().cuda()), "head dimension must match"),
+            (lambda: decode(k8=k8.half()), "int8 or float8_e4m3fn"),
+            (lambda: decode(v8=v8.view(torch.float8_e4m3fn)), "dtype of k_cache"),
+            (lambda: decode(v8=v8[:3].contiguous()), "same shape"),
+            (lambda: decode(scale=scale[:, :, 0].contiguous()), "kv_scale must be"),
+            (lambda: decode(table=table.long()), "2D int32"),
+            (lambda: decode(width=0), "must be positive"),
+            (lambda: decode(q=torch.zeros(2, 4, 1, D).half().cuda(), n=_ints([1, 1]).cuda(), table=_ints([[0], [1]]).cuda()), "row stride"),
+            (lambda: decode(n=n.long()), "seq_lens must be"),
+            (lambda: decode(softcap=-1.0), "softcap"),
+            (lambda: decode(softcap=math.nan), "softcap"),
+            (lambda: decode(mass=mass[:, :, :31].contiguous()), "room for every token"),
+            (lambda: decode(mass=mass.half()), "mass must be float32"),
+            (lambda: decode(mass=mass[:0]), "row for each sequence"),
+            (lambda: decode(mass_index=n), "goes with mass"),
+            (lambda: decode(q=torch.zeros(1, 4, 40000, D).half().cuda()), "query rows"),
+            (lambda: append(k=k.float(), v=k.float()), "k must be"),
+            (lambda: append(v=k.bfloat16()), "dtype and shape of k"),
+            (lambda: append(n=None), "positions is required"),
+            (lambda: append(k=k[:, :1].contiguous(), v=k[:, :1].contiguous()), "match k_cache in heads"),
+            (lambda: append(k=k.transpose(1, 3).contiguous().transpose(1, 3), v=k), "must be contiguous"),
+            (lambda: append(k=k, cu_seqlens=_ints([0, 1]).cuda()), "3D"),
+            (lambda: evict(budget=0), "budget"),
+            (lambda: evict(budget=33), "room for budget"),
+            (lambda: evict(sink=9, recent=8), "budget"),
+            (lambda: evict(mass=mass[:, :1].contiguous()), "mass must be")):
+        with pytest.raises(RuntimeError, match=message):
+            call()
+    rows = torch.zeros(3 * H * D + 4).half().cuda()
+    with pytest.raises(RuntimeError, match="multiples of 16 bytes"):
+        fa.append_paged_kv8(rows[4:].view(3, H, D), rows[4:].view(3, H, D), k8, v8, scale, table, None, 2, cu_seqlens=_ints([0, 3]).cuda())
