@@ -75,7 +75,7 @@ struct DecodeShape {
 DecodeShape decode_shape(int dim, int rows, int sms);
 cudaError_t launch_decode(DecodeArgs a, bool e4m3, cudaStream_t s);
 
-constexpr int kPlanHead = 4;
+constexpr int kPlanHead = 4;      // places of a large and of a small unit, small units taken
 constexpr int kMaxBatch = 4096;      // sequences of one launch: their page counts' running sum is kept in shared memory
 
 __device__ __forceinline__ bool page_ok(const Cache& c, int id) { return id >= 0 && id < c.pages; }

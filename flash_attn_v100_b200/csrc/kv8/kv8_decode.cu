@@ -14,10 +14,13 @@
 // The pages of all sequences and heads are cut evenly over the warps; where there are fewer segments than half the CTAs each is cut into equal
 // parts, at least kLeastPart pages, that the warps of a CTA share.  Parts of a cut segment go through global memory to a second launch, which, like the
 // first, is on its way before the launch in front of it has ended.
-// Measured: 64 sequences of 512 to 8192 tokens, 32 heads on 8 of 128, int8: 108.5 us for 573 MB, 5.3 TB/s (124 with loads straight to registers and an
-// even cut over CTAs).  Of it 8 us pass before the first codes are there, and the warps end between 65 and 98 us: some SMs get their bytes
-// a sixth later than others.  Looked at and left: L2 prefetches 2 to 6 steps ahead (slower by 5 to 14 %: nothing waits for DRAM alone), ranges for early
-// finishers, as CTAs of their own or taken over by running ones (the longer program costs what they gain), more CTAs than fit at once (12 us a wave).
+// Measured, int8, 32 heads on 8 of 128: 64 sequences of 512 to 8192 tokens 110 us for 573 MB (5.2 TB/s), one of 131071 (e4m3) 52.5 us for 269 MB; four of up to
+// 101 tokens 5.8 us.  Two CTAs of four warps an SM, 16 KB of ring each: with three the first takes as long, the second 57 us (bytes on their way are enough
+// with eight warps, and more wait longer for theirs).  Of the first case 4 us pass before the memory is busy and 5 behind the last code; between them it
+// delivers 7.3 TB/s until the first SMs are through, and the last are a sixth later: some get their bytes slower than others.  Looked at and left: loads
+// straight to registers (117), L2 prefetches 2 to 6 steps ahead (slower by 5 to 14 %), a quarter of the pages in small ranges for warps that are through
+// early, as CTAs of their own, taken over by running ones or counted out by an atomic (116 to 150: a new piece waits for its page numbers, its rows of q
+// and its codes in turn behind all bytes on their way), more CTAs than fit at once (12 us a wave).
 #include <math_constants.h>
 
 #include "kv8.cuh"
@@ -115,21 +118,62 @@ __device__ __forceinline__ int running_sum(int batch, int* first, int* warp_sums
   return total;
 }
 
+// The same by each warp for itself, f(b, the running sum before b) once it is known: all warps write the same, and none waits for another.
+template <class F, class G>
+__device__ __forceinline__ int running_sum_of_warp(int batch, F f, G g) {
+  const int lane = threadIdx.x & 31;
+  int total = 0;
+  for (int b0 = 0; b0 < batch; b0 += 32) {
+    const int v = b0 + lane < batch ? f(b0 + lane) : 0;
+    int x = v;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += y;
+    }
+    if (b0 + lane < batch) g(b0 + lane, total + x - v);
+    total += __shfl_sync(0xffffffffu, x, 31);
+  }
+  return total;
+}
+
+constexpr int kFewSequences = 128;      // up to which a warp is as fast alone as the block with its waits (64: 0.4 and 1.5 us)
+
 __device__ __forceinline__ Plan make_plan(const DecodeArgs& a, int* first, int* lens, int* warp_sums) {
   Plan p;
-  const int lanes = a.c.heads * a.blocks, segments = a.batch * lanes;
-  for (int b = threadIdx.x; b < a.batch; b += kThreads) lens[b] = min(max(a.lens[b], 0), a.c.max_pages * kPage);
-  __syncthreads();
-  const int opening = a.even ? kOpening : 0;
-  const int units = running_sum(a.batch, first, warp_sums, [&](int b) { return lens[b] ? (lens[b] + kPage - 1) / kPage + opening : 0; }) * lanes;
+  const int lanes = a.c.heads * a.blocks, segments = a.batch * lanes, most = a.c.max_pages * kPage;
+  const bool few = a.batch <= kFewSequences;
+  const auto places = [&](int len) { return len == 0 ? 0 : (len + kPage - 1) / kPage + (a.even ? kOpening : 0); };
+  const auto parts = [&](int b) { return ((lens[b] + kPage - 1) / kPage + p.per - 1) / p.per; };
+  int units;
+  if (few) {
+    units = running_sum_of_warp(a.batch, [&](int b) {
+      const int len = min(max(a.lens[b], 0), most);
+      lens[b] = len;
+      return places(len);
+    }, [&](int b, int before) { if (a.even) first[b] = before; });
+    if (a.even) first[a.batch] = units;
+  } else {
+    for (int b = threadIdx.x; b < a.batch; b += kThreads) lens[b] = min(max(a.lens[b], 0), most);
+    __syncthreads();
+    units = running_sum(a.batch, first, warp_sums, [&](int b) { return places(lens[b]); });
+  }
+  units *= lanes;
   if (a.even) {
     const int warps = a.n_cta * kWarps;
     p.per = max(1, (units + warps - 1) / warps);
   } else {
     // no more parts than CTAs: sum of ceil(pages / per) <= units / per + segments
     p.per = max(kLeastPart, (units + a.n_cta - segments - 1) / (a.n_cta - segments));
-    running_sum(a.batch, first, warp_sums + kWarps, [&](int b) { return ((lens[b] + kPage - 1) / kPage + p.per - 1) / p.per; });
+    if (few) {
+      __syncwarp();
+      const int total = running_sum_of_warp(a.batch, parts, [&](int b, int before) { first[b] = before; });
+      first[a.batch] = total;
+    } else {
+      running_sum(a.batch, first, warp_sums + kWarps, parts);
+    }
   }
+  __syncwarp();
   return p;
 }
 
@@ -156,7 +200,7 @@ struct Shape {
   static constexpr int kChunks = D / 64;       // 16-byte pieces of a key row that a lane takes
   static constexpr int kSteps = D / 16;        // of the contraction, and tiles of O^T
   static constexpr int kRows = NT * 8;
-  static constexpr int kCtas = D == 256 ? 2 : NT == 2 ? (D == 64 ? 3 : 2) : (D == 64 ? 4 : 3);
+  static constexpr int kCtas = D == 256 ? 2 : NT == 2 ? (D == 64 ? 3 : 2) : (D == 64 ? 4 : 2);
   static constexpr int kRing = kSlots * kTile * (2 * kPage * D + 8);      // bytes of a warp
   static constexpr int kMerge = kRows * (D + 4 + 2) * 4;            // what a warp hands over at the end of a shared piece, in the same place
   static constexpr int kWarpBytes = ((kRing > kMerge ? kRing : kMerge) + 127) / 128 * 128;
@@ -204,17 +248,6 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Plan plan = make_plan(a, first, lens, warp_sums);
-  if (blockIdx.x == 0) {
-    for (int i = tid; i <= a.batch; i += kThreads) a.plan[kPlanHead + i] = first[i];
-    if (tid == 0) a.plan[0] = plan.per;
-  }
-  // Sequences without keys.
-  for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
-    if (lens[b] != 0) continue;
-    const int64_t n = (int64_t)a.c.heads * a.rows * D;
-    uint16_t* o = static_cast<uint16_t*>(a.out) + b * n;
-    for (int64_t i = tid; i < n; i += kThreads) o[i] = 0;
-  }
   // even: every warp has a range of its own.  else: the warps of a CTA share its part.
   const int unit = a.even ? blockIdx.x * kWarps + warp : blockIdx.x;
   const int share = a.even ? 1 : kWarps, turn = a.even ? 0 : warp;
@@ -232,13 +265,13 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
     const int in = at - first[x.b] * lanes;
     if (a.even) {
       const int places = x.pages + kOpening, seg = in / places, before = in - seg * places;
-      x.h = seg / a.blocks;
+      x.h = a.blocks == 1 ? seg : seg / a.blocks;
       x.rb = seg - x.h * a.blocks;
       x.next = min(end, at + places - before);
       x.p0 = max(0, before - kOpening);
       x.p1 = before + x.next - at - kOpening;      // (<= p0: the range ends before the first page)
     } else {
-      const int parts = first[x.b + 1] - first[x.b], i = in / a.blocks;
+      const int parts = first[x.b + 1] - first[x.b], i = a.blocks == 1 ? in : in / a.blocks;
       x.rb = in - i * a.blocks;
       x.h = i / parts;
       const int part = i - x.h * parts;
@@ -341,13 +374,24 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
   int at = range0;
   if (at < end) {
     open();
-    x = locate(at);
+    x = f;
     load_q(x);
 #pragma unroll 1                                // (a longer program starts later)
     for (int i = 0; i < kSlots; ++i) {
       copy_keys(i);
       copy_values(i);
     }
+  }
+  if (blockIdx.x == 0) {
+    for (int i = tid; i <= a.batch; i += kThreads) a.plan[kPlanHead + i] = first[i];
+    if (tid == 0) a.plan[0] = plan.per;
+  }
+  // Sequences without keys, while the first codes are on their way.
+  for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+    if (lens[b] != 0) continue;
+    const int64_t n = (int64_t)a.c.heads * a.rows * D;
+    uint16_t* o = static_cast<uint16_t*>(a.out) + b * n;
+    for (int64_t i = tid; i < n; i += kThreads) o[i] = 0;
   }
   int at_slot = 0;
   while (at < end) {
