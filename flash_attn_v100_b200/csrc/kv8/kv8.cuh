@@ -40,7 +40,7 @@ struct DecodeArgs {
   const int* lens;
   int batch, rows, tokens;      // rows: query rows of a KV head, (heads of its group) x tokens
   bool bf16, capped;
-  float scale, cap, inv_cap;    // score scale, in base 2 without a cap
+  float scale, cap, inv_cap;    // score scale, in base 2 without a cap; cap in base 2, 2 log2 e / cap
   float* mass;
   const int* mass_index;
   int mass_rows, mass_cap;
@@ -83,11 +83,6 @@ __device__ __forceinline__ bool page_ok(const Cache& c, int id) { return id >= 0
 __device__ __forceinline__ uint4 load_stream16(const void* p) {
   uint4 r;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-  return r;
-}
-__device__ __forceinline__ uint2 load_stream8(const void* p) {
-  uint2 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
   return r;
 }
 

@@ -157,7 +157,7 @@ int fak_decode_paged(const FakCache* cache, const void* q, void* out, const int3
   a.rows = rows; a.tokens = tokens; a.bf16 = dtype == FAK_BF16; a.capped = softcap > 0.f;
   a.scale = (float)(a.capped ? root : root * log2e);
   a.cap = (float)(softcap * log2e);
-  a.inv_cap = a.capped ? 1.f / softcap : 0.f;
+  a.inv_cap = a.capped ? (float)(2.0 * log2e / softcap) : 0.f;
   a.n_cta = d.n_cta; a.blocks = d.blocks; a.score_cols = d.score_cols;
   a.plan = reinterpret_cast<int*>(base + w.plan);
   a.part = reinterpret_cast<float*>(base + w.part);

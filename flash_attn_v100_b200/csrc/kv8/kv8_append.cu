@@ -3,8 +3,8 @@
 // For each page, head and kind that gets rows: a = max |x| of the new rows, scale' = max(a / top, 2^-100, the scale before if the page has
 // rows already), code = round(x / scale').  Bound by HBM: a prompt's row of D values is read as 2 D bytes and written as D.  One warp takes a page of one head
 // and kind whole into registers (D bytes a lane), so the rows are read once; the largest magnitude is found on the 16-bit patterns two at a
-// time, where NaN is above infinity.  Measured: 16 prompts of 128 to 4096 tokens, 8 heads of 128, bf16 to e4m3: 39.4 us for 208 MB, 5.3 TB/s (44 with a
-// warp a kind and 64-bit divisions to find its place; six CTAs an SM: four 41.1 us, eight as many as six).
+// time, where NaN is above infinity.  Measured: 16 prompts of 128 to 4096 tokens, 8 heads of 128, bf16 to e4m3: 37.6 us for 208 MB, 5.5 TB/s (44 with a
+// warp a kind and 64-bit divisions to find its place; six CTAs an SM: with four 4 % more, with eight the same); one new token of 64 sequences 3.1.
 #include "kv8.cuh"
 
 namespace fa {
@@ -100,7 +100,9 @@ __global__ void __launch_bounds__(kWarps * 32, D == 256 ? 3 : 6) append_kernel(c
   const int h = blockIdx.y;
   const uint32_t job = blockIdx.x * kWarps + (threadIdx.x >> 5);
   const int64_t first = (int64_t)(SPLIT ? job >> 1 : job) * window;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (first >= a.total) return;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   // lane i < window: token first + i, and whether it is the first of a page's new rows
   const int t = (int)first + lane, total = (int)a.total;
   int page = 0, slot = 0, n = 0;
@@ -145,14 +147,17 @@ cudaError_t launch_append_d(const AppendArgs& a, bool bf16, cudaStream_t s) {
   const bool split = a.cu == nullptr;
   const int64_t windows = split ? 2 * a.total : (a.total + kPage - 1) / kPage;
   const dim3 grid((unsigned)((windows + kWarps - 1) / kWarps), (unsigned)a.c.heads);
-  if (split) {
-    if (bf16) append_kernel<D, E4M3, true, true><<<grid, kWarps * 32, 0, s>>>(a);
-    else append_kernel<D, E4M3, false, true><<<grid, kWarps * 32, 0, s>>>(a);
-  } else {
-    if (bf16) append_kernel<D, E4M3, true, false><<<grid, kWarps * 32, 0, s>>>(a);
-    else append_kernel<D, E4M3, false, false><<<grid, kWarps * 32, 0, s>>>(a);
-  }
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;      // (its blocks wait for the end of the launch in front)
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (split) return bf16 ? cudaLaunchKernelEx(&cfg, append_kernel<D, E4M3, true, true>, a) : cudaLaunchKernelEx(&cfg, append_kernel<D, E4M3, false, true>, a);
+  return bf16 ? cudaLaunchKernelEx(&cfg, append_kernel<D, E4M3, true, false>, a) : cudaLaunchKernelEx(&cfg, append_kernel<D, E4M3, false, false>, a);
 }
 
 }  // namespace

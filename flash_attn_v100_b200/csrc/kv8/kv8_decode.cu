@@ -14,7 +14,7 @@
 // The pages of all sequences and heads are cut evenly over the warps; where there are fewer segments than half the CTAs each is cut into equal
 // parts, at least kLeastPart pages, that the warps of a CTA share.  Parts of a cut segment go through global memory to a second launch, which, like the
 // first, is on its way before the launch in front of it has ended.
-// Measured, int8, 32 heads on 8 of 128: 64 sequences of 512 to 8192 tokens 110 us for 573 MB (5.2 TB/s), one of 131071 (e4m3) 52.5 us for 269 MB; four of up to
+// Measured, int8, 32 heads on 8 of 128: 64 sequences of 512 to 8192 tokens 111.6 us for 573 MB (5.1 TB/s), one of 131071 (e4m3) 52.5 us for 269 MB; four of up to
 // 101 tokens 5.8 us.  Two CTAs of four warps an SM, 16 KB of ring each: with three the first takes as long, the second 57 us (bytes on their way are enough
 // with eight warps, and more wait longer for theirs).  Of the first case 4 us pass before the memory is busy and 5 behind the last code; between them it
 // delivers 7.3 TB/s until the first SMs are through, and the last are a sixth later: some get their bytes slower than others.  Looked at and left: loads
@@ -39,6 +39,12 @@ __device__ __forceinline__ float log2_of(float x) {
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// cap tanh(x inv_cap) = cap (1 - 2 / (e^(2 x inv_cap) + 1)), off by less than 2^-21 cap; inv_cap comes times 2 log2 e.
+__device__ __forceinline__ float capped(float x, float cap, float inv_cap) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(fast_exp2(x * inv_cap) + 1.f));
+  return fmaf(-2.f * cap, r, cap);
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -49,8 +55,8 @@ __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// int8 codes are taken as fp16 1152 + code (0x6400 | (byte ^ 0x80)); for keys the 1152 stays in the product and its multiple of the query row's sum is
-// taken off the score.
+// int8 codes become fp16 as 1152 + code (0x6400 | (byte ^ 0x80)) less 1152, exactly.  (Left in the keys, and its multiple of the query row's sum taken off the score,
+// the 1152 cost the score seven bits: the weights' sums were off by up to 2e-5, where fp32 has 1e-6.)
 constexpr uint32_t kMagic = 0x64646464u, kBias2 = 0x64806480u;
 
 // Four codes of a key row as the two halves of a step's contraction.
@@ -60,8 +66,8 @@ __device__ __forceinline__ void key_pairs(uint32_t w, uint32_t& lo, uint32_t& hi
     asm("{.reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b;}" : "=r"(lo), "=r"(hi) : "r"(w));
   } else {
     w ^= 0x80808080u;
-    lo = __byte_perm(w, kMagic, 0x4140);
-    hi = __byte_perm(w, kMagic, 0x4342);
+    lo = sub2(__byte_perm(w, kMagic, 0x4140), kBias2);
+    hi = sub2(__byte_perm(w, kMagic, 0x4342), kBias2);
   }
 }
 // Bytes 0, 1 (high: 2, 3) of two tokens' words as fp16 pairs (token, next token).
@@ -140,7 +146,7 @@ __device__ __forceinline__ int running_sum_of_warp(int batch, F f, G g) {
 constexpr int kFewSequences = 128;      // up to which a warp is as fast alone as the block with its waits (64: 0.4 and 1.5 us)
 
 __device__ __forceinline__ Plan make_plan(const DecodeArgs& a, int* first, int* lens, int* warp_sums) {
-  Plan p;
+  Plan p = {1};
   const int lanes = a.c.heads * a.blocks, segments = a.batch * lanes, most = a.c.max_pages * kPage;
   const bool few = a.batch <= kFewSequences;
   const auto places = [&](int len) { return len == 0 ? 0 : (len + kPage - 1) / kPage + (a.even ? kOpening : 0); };
@@ -200,7 +206,7 @@ struct Shape {
   static constexpr int kChunks = D / 64;       // 16-byte pieces of a key row that a lane takes
   static constexpr int kSteps = D / 16;        // of the contraction, and tiles of O^T
   static constexpr int kRows = NT * 8;
-  static constexpr int kCtas = D == 256 ? 2 : NT == 2 ? (D == 64 ? 3 : 2) : (D == 64 ? 4 : 2);
+  static constexpr int kCtas = D == 64 ? (NT == 2 ? 3 : 4) : 2;
   static constexpr int kRing = kSlots * kTile * (2 * kPage * D + 8);      // bytes of a warp
   static constexpr int kMerge = kRows * (D + 4 + 2) * 4;            // what a warp hands over at the end of a shared piece, in the same place
   static constexpr int kWarpBytes = ((kRing > kMerge ? kRing : kMerge) + 127) / 128 * 128;
@@ -404,11 +410,11 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
     const int64_t head = (int64_t)b * a.c.heads + h;
     // ---- query rows as the second operand, fp16; bf16 rows are brought into its range by a power of two
     uint32_t qf[NT][kSteps][2];
-    float factor[NT][2], offset[NT][2];         // of the lane's columns 2t and 2t + 1
+    float factor[NT][2];                        // of the lane's columns 2t and 2t + 1
     int limit[NT][2];                           // keys that they see
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float sum = 0.f, up = 1.f;
+      float up = 1.f;
       uint32_t raw[kSteps][2];
 #pragma unroll
       for (int c = 0; c < kChunks; ++c)
@@ -434,21 +440,13 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
             raw[i][j] = pack_half2(__uint_as_float(raw[i][j] << 16) * down, __uint_as_float(raw[i][j] & 0xffff0000u) * down);
       }
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          qf[n][i][j] = raw[i][j];
-          if constexpr (!E4M3) {
-            const float2 f = __half22float2(*reinterpret_cast<__half2*>(&raw[i][j]));
-            sum += f.x + f.y;
-          }
-        }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      for (int i = 0; i < kSteps; ++i) {
+        qf[n][i][0] = raw[i][0];
+        qf[n][i][1] = raw[i][1];
+      }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int col = n * 8 + 2 * t + c;
-        offset[n][c] = E4M3 ? 0.f : -1152.f * __shfl_sync(0xffffffffu, sum, (2 * t + c) * 4);
         factor[n][c] = a.scale * __shfl_sync(0xffffffffu, up, (2 * t + c) * 4);
         limit[n][c] = col < rows ? len - a.tokens + 1 + (r0 + col) % a.tokens : 0;
       }
@@ -509,14 +507,14 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[u][n][e] = (s[u][n][e] + offset[n][e & 1]) * (factor[n][e & 1] * ks[u]);
+          for (int e = 0; e < 4; ++e) s[u][n][e] *= factor[n][e & 1] * ks[u];
       if (a.capped) {
 #pragma unroll
         for (int u = 0; u < kTile; ++u)
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[u][n][e] = a.cap * tanhf(s[u][n][e] * a.inv_cap);
+            for (int e = 0; e < 4; ++e) s[u][n][e] = capped(s[u][n][e], a.cap, a.inv_cap);
       }
       const bool masked = key0 + kTile * kPage > free_keys || base + kTile > p1;
       if (masked) {
@@ -909,12 +907,18 @@ constexpr int ctas_of() { return Shape<D, NT>::kCtas; }
 
 }  // namespace
 
+// Query rows of a block: 8, or 16 for more of up to 128 columns.  What is in a block reads every code once, another block reads it again (mostly from L2).
+// Blocks of 32 for width 64 were slower, 39 to 48 us against 33 for 20 rows each of 16 sequences of up to 4096 tokens: their registers leave too little
+// under way at once.
+static int tiles_of(int dim, int rows) { return dim == 256 || rows <= 8 ? 1 : 2; }
+
 DecodeShape decode_shape(int dim, int rows, int sms) {
   DecodeShape d;
-  const bool wide = rows > 8 && dim <= 128;
-  d.row_block = wide ? 16 : 8;
+  const int tiles = tiles_of(dim, rows);
+  d.row_block = tiles * 8;
   d.blocks = (rows + d.row_block - 1) / d.row_block;
-  const int ctas = dim == 64 ? (wide ? ctas_of<64, 2>() : ctas_of<64, 1>()) : dim == 128 ? (wide ? ctas_of<128, 2>() : ctas_of<128, 1>()) : ctas_of<256, 1>();
+  const int ctas = dim == 256 ? ctas_of<256, 1>() : dim == 128 ? (tiles == 2 ? ctas_of<128, 2>() : ctas_of<128, 1>())
+                 : tiles == 2 ? ctas_of<64, 2>() : ctas_of<64, 1>();
   d.n_cta = sms * ctas;
   d.slots = 2 * d.n_cta * kWarps;
   d.score_cols = rows >= d.row_block ? d.row_block : (rows + 1) & ~1;
@@ -923,10 +927,10 @@ DecodeShape decode_shape(int dim, int rows, int sms) {
 
 cudaError_t launch_decode(DecodeArgs a, bool e4m3, cudaStream_t s) {
   a.even = 2 * (int64_t)a.batch * a.c.heads * a.blocks > a.n_cta;
-  const bool wide = a.rows > 8 && a.c.dim <= 128;
+  const int tiles = tiles_of(a.c.dim, a.rows);
   switch (a.c.dim) {
-    case 64: return wide ? launch_decode_codes<64, 2>(a, e4m3, s) : launch_decode_codes<64, 1>(a, e4m3, s);
-    case 128: return wide ? launch_decode_codes<128, 2>(a, e4m3, s) : launch_decode_codes<128, 1>(a, e4m3, s);
+    case 64: return tiles == 2 ? launch_decode_codes<64, 2>(a, e4m3, s) : launch_decode_codes<64, 1>(a, e4m3, s);
+    case 128: return tiles == 2 ? launch_decode_codes<128, 2>(a, e4m3, s) : launch_decode_codes<128, 1>(a, e4m3, s);
     default: return launch_decode_codes<256, 1>(a, e4m3, s);
   }
 }

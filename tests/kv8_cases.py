@@ -47,11 +47,11 @@ def decode_bound(q, k_cache, scale, out, size, dtype, softcap):
 
     The rounding of the result; of every weight to fp16 (2^-11 of its product with the value, 2^-24 of the largest value
     where a weight is below fp16's normal range); and what the score's error does to numerator and denominator.  Scores add D / 16 products of
-    tensor cores in fp32, each sum off by at most 2^-22 of sum |q| times the largest operand, 1152 + 127 for int8 codes (the offset they carry), 448 for
-    e4m3; base-2 exponentials, the cap's tanh and the multiplications: 2^-18 and 2^-21 of the cap."""
+    tensor cores in fp32, each sum off by at most 2^-22 of sum |q| times the largest code, 127 or 448; base-2 exponentials, the cap's tanh and the
+    multiplications: 2^-18 and 2^-21 of the cap."""
     D = q.shape[3]
-    most = 1279.0 if k_cache.dtype == torch.int8 else 448.0
+    most = orc.TOP[k_cache.dtype]
     score = float(q.double().abs().sum(3).max()) * most * float(scale[..., 0].max()) / math.sqrt(D) * (D / 16) * 2.0 ** -22
     delta = score + softcap * 2.0 ** -21 + 2.0 ** -18
-    assert delta < 2.0 ** -6
+    assert delta < 2.0 ** -7
     return out.abs() * half_step(dtype) + size * (2.0 ** -11 + 2 * delta) + float(size.max()) * 2.0 ** -20, delta
