@@ -406,7 +406,7 @@ PyObject* kv8_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const double softcap = PyFloat_AS_DOUBLE(a[7]);
   const at::Tensor* q = c.tensor(a[0], type, 4);
   const int width = c.integer(a[6]);
-  c.need(softcap >= 0.0 && softcap <= 1e30);
+  c.need(softcap == 0.0 || (softcap >= 1e-30 && softcap <= 1e30));
   if (!c.ok) Py_RETURN_NONE;
   const int64_t batch = q->size(0), heads = q->size(1), tokens = q->size(2);
   FakCache cache;

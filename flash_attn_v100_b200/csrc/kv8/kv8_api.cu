@@ -137,7 +137,7 @@ int fak_decode_paged(const FakCache* cache, const void* q, void* out, const int3
   int rc = check_decode(cache, batch, q_heads, tokens);
   if (rc != FAK_OK) return rc;
   FA_REQUIRE(dtype_ok(dtype), "unknown dtype %d", dtype);
-  FA_REQUIRE(softcap >= 0.f && softcap <= 1e30f, "softcap must be finite and not negative");
+  FA_REQUIRE(softcap == 0.f || (softcap >= 1e-30f && softcap <= 1e30f), "softcap must be 0 or from 1e-30 to 1e30");
   if (batch == 0) return FAK_OK;
   FA_REQUIRE(q && out && lens && workspace, "null pointer");
   FA_REQUIRE(aligned16(q) && aligned16(out) && aligned16(workspace), "q, out and the workspace must be 16-byte aligned");

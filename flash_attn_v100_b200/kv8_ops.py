@@ -1,7 +1,7 @@
 """Operators on a paged cache in 8 bits (include/fa_b200_kv8.h): what writes it, what reads it and what makes it shorter.
 
 The cache keeps 16 tokens a page: k_cache and v_cache [pages, H_KV, 16, D], int8 (codes -127..127) or float8_e4m3fn, and kv_scale [pages, H_KV, 2]
-fp32 with a scale for each page, head and kind (0: keys, 1: values); a code stands for code * scale.  D is 64, 128 or 256.  block_table [B, *] int32
+fp32 with a scale for each page, head and kind (0: keys, 1: values), up to 2^60; a code stands for code * scale.  D is 64, 128 or 256.  block_table [B, *] int32
 with row stride `max_num_blocks` holds a sequence's pages in order, as in `forward_paged_decode_gqa_fp16`.  q, k, v are float16 or bfloat16.
 
 Calls go to the current stream of the tensors' device and can be captured in CUDA graphs; there is no CPU path.  A page outside the
@@ -136,7 +136,7 @@ def forward_paged_decode_gqa_kv8(q, k_cache, v_cache, kv_scale, block_table, seq
     q [B,H_Q,T,D], seq_lens [B] int32 (the T tokens counted in) -> new [B,H_Q,T,D].  Token t sees the keys before seq_len - T + t + 1; one that
     sees none gets zeros.  With softcap > 0 a score x becomes softcap * tanh(x / softcap).  `mass` [rows,H_KV,tokens] fp32: what every key
     is given by the softmax, summed over the query heads of its KV head and the T tokens, is added in place to row mass_index[b] (None: b); the
-    rows of a call must be different ones."""
+    rows of a call must be different ones.  It takes 4 bytes of scratch for every query row and token that a block_table row has room for."""
     done = _native("kv8_decode", q, k_cache, v_cache, kv_scale, block_table, seq_lens, max_num_blocks, softcap, mass, mass_index)
     if done is not None:
         return done
@@ -151,7 +151,7 @@ def forward_paged_decode_gqa_kv8(q, k_cache, v_cache, kv_scale, block_table, seq
     _chk(T > 0, "q must have at least one token")
     _ints(seq_lens, "seq_lens", batch, k_cache)
     softcap = float(softcap)
-    _chk(0.0 <= softcap <= 1e30, "softcap must be finite and not negative")
+    _chk(softcap == 0.0 or 1e-30 <= softcap <= 1e30, "softcap must be 0 or from 1e-30 to 1e30")
     if mass is not None:
         _check_mass(mass, mass_index, batch, c, k_cache)
     else:

@@ -386,7 +386,7 @@ class PagedKVCache8(BlockManager):
 
     def evict(self, request_ids: Sequence[str], budget: int, sink: int = 4, recent: int = 64) -> int:
         """Cut every request of more than `budget` committed tokens to `budget`, layer by layer and head by head; returns the blocks
-        that came free.  The tokens move to new blocks, so blocks that other requests or a prefix share stay as they are; there must
+        that came free (less than 0 where shared ones stay held).  The tokens move to new blocks, so blocks that other requests or a prefix share stay as they are; there must
         be enough free ones for the requests that are cut."""
         from . import kv8_ops
         if self.masses is None:
@@ -402,15 +402,20 @@ class PagedKVCache8(BlockManager):
         n = (budget + BLOCK_SIZE - 1) // BLOCK_SIZE
         blocks = self._take_blocks(n * len(ids))
         new = [blocks[i * n: (i + 1) * n] for i in range(len(ids))]
-        table, lens = self.batch_view(ids)
-        new_table = torch.tensor(new, dtype=torch.int32).to(self.device)
-        rows = torch.tensor([self._row[r] for r in ids], dtype=torch.int32).to(self.device)
-        at = rows.long()
-        for layer in range(self.num_layers):
-            mass = self.masses[layer]
-            _, _, kept = kv8_ops.evict_paged_kv8(mass, self.k_pools[layer], self.v_pools[layer], self.scales[layer], table, lens,
-                                                 self.max_blocks_per_seq, new_table, budget, sink, recent, mass_index=rows)
-            mass[at] = torch.nn.functional.pad(kept, (0, mass.size(2) - budget))
+        try:
+            table, lens = self.batch_view(ids)
+            new_table = torch.tensor(new, dtype=torch.int32).to(self.device)
+            rows = torch.tensor([self._row[r] for r in ids], dtype=torch.int32).to(self.device)
+            at = rows.long()
+            for layer in range(self.num_layers):
+                mass = self.masses[layer]
+                _, _, kept = kv8_ops.evict_paged_kv8(mass, self.k_pools[layer], self.v_pools[layer], self.scales[layer], table, lens,
+                                                     self.max_blocks_per_seq, new_table, budget, sink, recent, mass_index=rows)
+                mass[at] = torch.nn.functional.pad(kept, (0, mass.size(2) - budget))
+        except Exception:
+            for b in reversed(blocks):
+                self._drop_ref(b)
+            raise
         for r, own in zip(ids, new):
             row, old = self._row[r], self._tables[r]
             self._tables[r] = list(own)

@@ -47,8 +47,8 @@ int fak_append_paged(const FakCache* cache, const void* k, const void* v, int64_
                      const int32_t* cu_seqlens, int batch, int64_t total, void* stream);
 
 /* Attention of the `tokens` newest tokens of each sequence, q and out [batch, q_heads, tokens, dim]; lens [batch] counts them in.  Token t of
- * a sequence sees the keys before lens - tokens + t + 1; a row that sees none gives zeros.  Scores (q . k) / sqrt(dim), with softcap > 0
- * softcap * tanh(score / softcap).  mass [mass_rows, heads, mass_cap] fp32, where given: every key's weights, summed over the rows of its head, are added to row
+ * a sequence sees the keys before lens - tokens + t + 1; a row that sees none gives zeros.  Scores (q . k) / sqrt(dim), with softcap (0, or
+ * from 1e-30 to 1e30) softcap * tanh(score / softcap).  mass [mass_rows, heads, mass_cap] fp32, where given: every key's weights, summed over the rows of its head, are added to row
  * mass_index[b] (null: b), which must be another one for each b.  The workspace (16-byte aligned) has fak_decode_workspace bytes. */
 size_t fak_decode_workspace(const FakCache* cache, int batch, int q_heads, int tokens, int with_mass);
 int fak_decode_paged(const FakCache* cache, const void* q, void* out, const int32_t* lens, int batch, int q_heads, int tokens, int dtype, float softcap,

@@ -1,6 +1,9 @@
 """GPU: the operators on the paged 8-bit cache against the CPU oracle.  Codes, scales, kept tokens and their sums are compared bit for bit;
 attention goes by the bound that tests/kv8_cases.py derives."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -10,6 +13,7 @@ from oracle import kv8_oracle as orc
 
 pytestmark = pytest.mark.gpu
 CODES = kc.CODES
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 @pytest.fixture(scope="module")
@@ -486,6 +490,32 @@ def test_calls_on_another_stream_and_in_a_graph(fa):
             s["lens"].add_(1); s["pos"].add_(1)
 
 
+FIRST_CALL_IN_A_GRAPH = """
+import torch
+import flash_attn_v100_b200 as fa
+k8, v8 = (torch.ones(4, 2, 16, 64, dtype=torch.int8, device="cuda") for _ in range(2))
+scale, table, lens = torch.ones(4, 2, 2, device="cuda"), torch.arange(4, device="cuda").int()[None], torch.full((1,), 50, device="cuda").int()
+k, q = torch.full((1, 2, 1, 64), 2.0, device="cuda").half(), torch.zeros(1, 4, 1, 64, device="cuda").half()
+mass, new = torch.zeros(1, 2, 64, device="cuda"), torch.arange(2, 4, device="cuda").int()[None]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    fa.append_paged_kv8(k, k, k8, v8, scale, table, lens - 1, 4)
+    out = fa.forward_paged_decode_gqa_kv8(q, k8, v8, scale, table, lens, 4, mass=mass)
+    kept, n, _ = fa.evict_paged_kv8(mass, k8, v8, scale, table[:, :2].contiguous(), lens - 18, 2, new, 20)
+graph.replay()
+torch.cuda.synchronize()
+fa.check_async_errors()
+assert torch.allclose(out.float(), torch.full_like(out, 1 + 1 / 50).float(), atol=1e-3), out
+assert abs(mass.sum().item() - 4) < 1e-3 and n.item() == 20 and kept[0, 0].tolist() == list(range(20))
+print("fine")
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    run = subprocess.run([sys.executable, "-c", FIRST_CALL_IN_A_GRAPH], capture_output=True, text=True, timeout=120, cwd=ROOT)
+    assert run.returncode == 0 and "fine" in run.stdout, run.stderr[-2000:]
+
+
 def test_results_do_not_change_from_call_to_call(fa):
     lens = [3000, 17, 900]
     table, _ = kc.tables(lens, 260, 96)
@@ -629,6 +659,7 @@ def test_calls_that_do_not_fit_are_refused(fa):
             (lambda: decode(n=n.long()), "seq_lens must be"),
             (lambda: decode(softcap=-1.0), "softcap"),
             (lambda: decode(softcap=math.nan), "softcap"),
+            (lambda: decode(softcap=1e-40), "softcap"),
             (lambda: decode(mass=mass[:, :, :31].contiguous()), "room for every token"),
             (lambda: decode(mass=mass.half()), "mass must be float32"),
             (lambda: decode(mass=mass[:0]), "row for each sequence"),

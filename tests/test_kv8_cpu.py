@@ -47,7 +47,7 @@ def test_refusals_before_the_device(lib):
     assert append(_cache(), total=0, batch=0) == 0
     decode = lambda c, q_heads=4, tokens=1, cap=0.0, mass=None, rows=0, cap_m=0, ws=p, n=1 << 40, dtype=0: lib.fak_decode_paged(
         ref(c), p, p, p, 1, q_heads, tokens, dtype, cap, mass, None, rows, cap_m, ws, n, None)
-    for bad in (dict(q_heads=3), dict(q_heads=0), dict(tokens=0), dict(cap=-1.0), dict(cap=math.inf), dict(cap=math.nan), dict(mass=p), dict(ws=None), dict(n=16),
+    for bad in (dict(q_heads=3), dict(q_heads=0), dict(tokens=0), dict(cap=-1.0), dict(cap=1e-31), dict(cap=math.inf), dict(cap=math.nan), dict(mass=p), dict(ws=None), dict(n=16),
                 dict(dtype=7), dict(ws=ctypes.c_void_p(264)), dict(tokens=65536)):
         assert decode(_cache(), **bad) == -1, bad
     assert b"query rows" in lib.fak_last_error()
@@ -131,6 +131,9 @@ def test_cache_class_bookkeeping():
         c.evict(["b"], 60, 0, 0)                                  # four new blocks are needed
     assert c.get_num_free_blocks() == free and c.get_cache_len("b") == 64
     c.release("a")
+    with pytest.raises(RuntimeError):
+        c.evict(["b"], 30, 0, 0)                                  # (no kernel on the CPU: the new blocks go back)
+    assert c.get_num_free_blocks() == free + 2 and c.get_cache_len("b") == 64 and c.position("b") == 64
     with pytest.raises(KeyError):
         c.position("a")
     with pytest.raises(RuntimeError, match="no sums"):
