@@ -9,18 +9,20 @@
 // runs ahead of its own reads from one piece into the next.  A lane's 16 bytes of a key row are four steps of the (permuted) contraction, and its 16
 // bytes of four tokens' values the rows of eight tiles of O^T.  They become fp16 in registers, exactly.
 // K's scale multiplies the finished scores.  V's scale goes into the exponent: with m the running maximum of s + log2 vs the weight that meets the
-// codes is 2^(s + log2 vs - m) <= 1, so fp16 keeps 11 bits of the products that matter whatever the pages' scales are; the sum of weights
+// codes is 2^(s - m) vs <= 1, so fp16 keeps 11 bits of the products that matter whatever the pages' scales are; the sum of weights
 // takes 2^(s - m) in fp32.
 // The pages of all sequences and heads are cut evenly over the warps; where there are fewer segments than half the CTAs each is cut into equal
 // parts, at least kLeastPart pages, that the warps of a CTA share.  Parts of a cut segment go through global memory to a second launch, which, like the
 // first, is on its way before the launch in front of it has ended.
-// Measured, int8, 32 heads on 8 of 128: 64 sequences of 512 to 8192 tokens 111.6 us for 573 MB (5.1 TB/s), one of 131071 (e4m3) 52.5 us for 269 MB; four of up to
-// 101 tokens 5.8 us.  Two CTAs of four warps an SM, 16 KB of ring each: with three the first takes as long, the second 57 us (bytes on their way are enough
+// Measured, int8, 32 heads on 8 of 128: 64 sequences of 512 to 8192 tokens 110.8 us for 573 MB (5.2 TB/s), one of 131071 (e4m3) 51.3 us for 269 MB; four of up to
+// 101 tokens 5.7 us.  Two CTAs of four warps an SM, 16 KB of ring each: with three the first takes as long, the second 57 us (bytes on their way are enough
 // with eight warps, and more wait longer for theirs).  Of the first case 4 us pass before the memory is busy and 5 behind the last code; between them it
 // delivers 7.3 TB/s until the first SMs are through, and the last are a sixth later: some get their bytes slower than others.  Looked at and left: loads
 // straight to registers (117), L2 prefetches 2 to 6 steps ahead (slower by 5 to 14 %), a quarter of the pages in small ranges for warps that are through
 // early, as CTAs of their own, taken over by running ones or counted out by an atomic (116 to 150: a new piece waits for its page numbers, its rows of q
-// and its codes in turn behind all bytes on their way), more CTAs than fit at once (12 us a wave).
+// and its codes in turn behind all bytes on their way), more CTAs than fit at once (12 us a wave), keys as they are in three products with whole-numbered
+// parts of q (mma.s8: no conversion, the same time; 37 instead of 32 us for 20 rows of 16 sequences).  Of a step's 2600 cycles 50 are waits for codes and 880
+// the issue of the next copies, which is where a full memory system makes itself felt.
 #include <math_constants.h>
 
 #include "kv8.cuh"
@@ -303,6 +305,13 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
     const int p = f.p0 + (turn + share * (i0 + lane / kTile)) * kTile + lane % kTile;
     return p < f.p1 ? f_table[p] : 0;
   };
+  const auto adopt = [&](int id) {              // -1: none of the cache's, which is recorded and spoils what sees the page
+    if (!page_ok(a.c, id)) {
+      atomicOr(a.c.status, kStatusBadPageId);
+      id = -1;
+    }
+    return id;
+  };
   const auto open = [&] {                       // (only the last piece of a range can be without pages: it then ends the range)
     f = locate(f_at);
     f_at = f.next;
@@ -315,29 +324,33 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
     if (lane < min(kRows, a.rows - f.rb * kRows) * (D / 64))
       asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint16_t*>(a.q) + q0 + lane * 64));
   };
+  // Where a lane's pieces of rows go: the places repeat after kKinds copies, 512 bytes each.
+  constexpr int kKinds = D == 256 ? 4 : 2;
+  uint32_t key_to[kKinds], value_to[kKinds];
+#pragma unroll
+  for (int c = 0; c < kKinds; ++c) {
+    key_to[c] = mine_at + key_at<D>(c * (32 / kLanesRow) + lane / kLanesRow, lane % kLanesRow);
+    value_to[c] = mine_at + kTile * kPageBytes + value_at<D>(c * (32 / kLanesRow) + lane / kLanesRow, lane % kLanesRow);
+  }
+  const auto copy_page = [&](const uint32_t (&to)[kKinds], int slot, int u, const uint8_t* from) {
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) copy16(to[c % kKinds] + slot * (2 * kTile * kPageBytes) + u * kPageBytes + c / kKinds * (kKinds * 512), from + c * 512);
+  };
   const auto copy_keys = [&](int slot) {
     if (f_i < f.steps) {
-      const int base = f.p0 + (turn + share * f_i) * kTile;
+      const int base = f.p0 + (turn + share * f_i) * kTile, j = f_i % kAhead * kTile;
+      if (j == 0) f_id = adopt(f_id);
+      const int64_t head_at = (int64_t)f.h * kPageBytes + lane * 16;
+      const int own = __shfl_sync(0xffffffffu, f_id, j + lane % kTile);
 #pragma unroll
       for (int u = 0; u < kTile; ++u) {
-        pg[u] = __shfl_sync(0xffffffffu, f_id, f_i % kAhead * kTile + u);
-        if (base + u < f.p1) {
-          const bool fine = page_ok(a.c, pg[u]);
-          if (!fine) pg[u] = 0;
-          const uint8_t* from = a.c.k + pg[u] * page_bytes + f.h * kPageBytes + lane * 16;
-#pragma unroll
-          for (int c = 0; c < kCopies; ++c)
-            copy16(mine_at + (slot * 2 * kTile + u) * kPageBytes + key_at<D>(c * (32 / kLanesRow) + lane / kLanesRow, lane % kLanesRow), from + c * 512);
-          if (lane == u) {
-            const uint32_t to = scales_at + (slot * kTile + u) * 8;
-            if (fine) {
-              asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(a.c.scale + ((int64_t)pg[u] * a.c.heads + f.h) * 2) : "memory");
-            } else {
-              atomicOr(a.c.status, kStatusBadPageId);
-              asm volatile("st.shared.v2.f32 [%0], {%1, %1};" ::"r"(to), "f"(CUDART_NAN_F) : "memory");
-            }
-          }
-        }
+        pg[u] = max(0, __shfl_sync(0xffffffffu, f_id, j + u));
+        if (base + u < f.p1) copy_page(key_to, slot, u, a.c.k + pg[u] * page_bytes + head_at);
+      }
+      if (lane < kTile && base + lane < f.p1) {
+        const uint32_t to = scales_at + (slot * kTile + lane) * 8;
+        if (own >= 0) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(a.c.scale + ((int64_t)own * a.c.heads + f.h) * 2) : "memory");
+        else asm volatile("st.shared.v2.f32 [%0], {%1, %1};" ::"r"(to), "f"(CUDART_NAN_F) : "memory");
       }
     }
     cp_async_commit();
@@ -345,14 +358,10 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
   const auto copy_values = [&](int slot) {
     if (f_i < f.steps) {
       const int base = f.p0 + (turn + share * f_i) * kTile;
+      const int64_t head_at = (int64_t)f.h * kPageBytes + lane * 16;
 #pragma unroll
       for (int u = 0; u < kTile; ++u)
-        if (base + u < f.p1) {
-          const uint8_t* from = a.c.v + pg[u] * page_bytes + f.h * kPageBytes + lane * 16;
-#pragma unroll
-          for (int c = 0; c < kCopies; ++c)
-            copy16(mine_at + ((slot * 2 + 1) * kTile + u) * kPageBytes + value_at<D>(c * (32 / kLanesRow) + lane / kLanesRow, lane % kLanesRow), from + c * 512);
-        }
+        if (base + u < f.p1) copy_page(value_to, slot, u, a.c.v + pg[u] * page_bytes + head_at);
       ++f_i;
       if (f_i == f.steps) {
         if (f_at < end) open();
@@ -468,13 +477,12 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
       const int base = p0 + (turn + share * i) * kTile;
       cp_async_wait<2 * kSlots - 1>();
       __syncwarp();
-      float ks[kTile], lv[kTile];
+      float ks[kTile], vs[kTile];
 #pragma unroll
       for (int u = 0; u < kTile; ++u) {
-        float vs;
-        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(ks[u]), "=f"(vs) : "r"(scales_at + (at_slot * kTile + u) * 8));
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(ks[u]), "=f"(vs[u]) : "r"(scales_at + (at_slot * kTile + u) * 8));
         if (!(fabsf(ks[u]) <= 3.4028235e38f)) ks[u] = CUDART_NAN_F;      // a scale that is not finite spoils what sees the page, whatever the codes
-        lv[u] = base + u < p1 ? log2_of(vs) : 0.f;
+        if (base + u >= p1) vs[u] = 0.f;
       }
       // ---- S^T = K Q^T
       float s[kTile][NT][4];
@@ -544,31 +552,43 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
       // ---- running maximum of s + log2 vs
       uint32_t pf[kTile][NT][2];
       bool moved = false;
-      float shrink[NT][2];
+      float top[NT][2], lv[kTile];
+#pragma unroll
+      for (int u = 0; u < kTile; ++u) lv[u] = fminf(fmaxf(log2_of(vs[u]), -60.f), 60.f);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float x = -CUDART_INF_F;
+          float y = -CUDART_INF_F;
 #pragma unroll
-          for (int u = 0; u < kTile; ++u) x = fmaxf(x, fmaxf(s[u][n][c], s[u][n][c + 2]) + fminf(fmaxf(lv[u], -60.f), 60.f));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          const float top = fmaxf(m[n][c], x);
-          shrink[n][c] = top == -CUDART_INF_F ? 1.f : fast_exp2(m[n][c] - top);
-          moved |= top != m[n][c];
-          m[n][c] = top;
+          for (int u = 0; u < kTile; ++u) y = fmaxf(y, fmaxf(s[u][n][c], s[u][n][c + 2]) + lv[u]);
+          top[n][c] = y;
         }
+#pragma unroll
+      for (int d = 4; d < 32; d *= 2)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) top[n][c] = fmaxf(top[n][c], __shfl_xor_sync(0xffffffffu, top[n][c], d));
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) moved |= top[n][c] > m[n][c];
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          l[n][0] *= shrink[n][0];
-          l[n][1] *= shrink[n][1];
+          float shrink[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            top[n][c] = fmaxf(m[n][c], top[n][c]);
+            shrink[c] = top[n][c] == -CUDART_INF_F ? 1.f : fast_exp2(m[n][c] - top[n][c]);
+            m[n][c] = top[n][c];
+            l[n][c] *= shrink[c];
+          }
 #pragma unroll
           for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][k][e] *= shrink[n][e & 1];
+            for (int e = 0; e < 4; ++e) o[n][k][e] *= shrink[e & 1];
         }
       }
 #pragma unroll
@@ -576,15 +596,14 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
         const float ref[2] = {m[n][0] == -CUDART_INF_F ? 0.f : m[n][0], m[n][1] == -CUDART_INF_F ? 0.f : m[n][1]};
 #pragma unroll
         for (int u = 0; u < kTile; ++u) {
-          float p[4];
+          float p[4];                             // (at most 2^60, and times vs at most 1)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float d = s[u][n][e] - ref[e & 1];
-            l[n][e & 1] += fast_exp2(d);
-            p[e] = fast_exp2(d + lv[u]);
+            p[e] = fast_exp2(s[u][n][e] - ref[e & 1]);
+            l[n][e & 1] += p[e];
           }
-          pf[u][n][0] = transpose8x8(pack_half2(p[0], p[1]));
-          pf[u][n][1] = transpose8x8(pack_half2(p[2], p[3]));
+          pf[u][n][0] = transpose8x8(pack_half2(p[0] * vs[u], p[1] * vs[u]));
+          pf[u][n][1] = transpose8x8(pack_half2(p[2] * vs[u], p[3] * vs[u]));
         }
       }
       // ---- O^T += V^T P^T
