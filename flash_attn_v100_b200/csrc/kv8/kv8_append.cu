@@ -114,14 +114,15 @@ __global__ void __launch_bounds__(kWarps * 32, D == 256 ? 3 : 6) append_kernel(c
       begin = a.cu[b];
       end = min(a.cu[b + 1], total);
     }
-    if (t >= begin && t < end && begin >= 0) {
-      const int64_t pos = (int64_t)(a.positions != nullptr ? a.positions[b] : 0) + (t - begin);
+    const int start = a.positions != nullptr ? a.positions[b] : 0;      // (negative: a row of a padded batch)
+    if (t >= begin && t < end && begin >= 0 && start >= 0) {
+      const int64_t pos = (int64_t)start + (t - begin);
       slot = (int)pos & (kPage - 1);
       leads = t == begin || slot == 0;
       n = min(kPage - slot, end - t);
       const int64_t index = pos >> 4;
       page = -1;
-      if (leads && pos >= 0 && index < a.c.max_pages) page = a.c.table[(int64_t)b * a.c.width + index];
+      if (leads && index < a.c.max_pages) page = a.c.table[(int64_t)b * a.c.width + index];
       if (leads && !page_ok(a.c, page)) {
         atomicOr(a.c.status, kStatusBadPageId);
         leads = false;

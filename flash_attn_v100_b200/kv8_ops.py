@@ -82,7 +82,8 @@ def append_paged_kv8(k, v, k_cache, v_cache, kv_scale, block_table, positions, m
     """New keys and values into the pages of an 8-bit cache, in place.
 
     Decode step (cu_seqlens is None): k, v [B,H_KV,1,D]; positions [B] int32 = slot of the new token.  Packed prompts: k, v [total,H_KV,D],
-    cu_seqlens [B+1] int32; token j of sequence s is stored at slot positions[s] + j (positions None = 0).  The tokens of k and v may be any
+    cu_seqlens [B+1] int32; token j of sequence s is stored at slot positions[s] + j (positions None = 0).  A sequence
+    with a negative position is left out (padded batches; attention takes a seq_len of 0 for it).  The tokens of k and v may be any
     multiple of 8 elements apart (slices of a fused projection).  Per page, head and kind: the scale is the largest magnitude of its rows / 127
     (e4m3: 448), at least 2^-100.  Where a page goes on being filled its scale only grows, and the codes it has are then rounded again.  NaN and
     infinities make a page's scale infinite, and what attends to it NaN.  Two sequences of a call must not write to the same page."""

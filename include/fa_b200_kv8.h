@@ -39,7 +39,8 @@ int fak_status(void* stream, int* status, int clear);
 uint64_t fak_devices(void);
 
 /* New rows into pages.  k, v: `total` tokens of [heads, dim], k_stride and v_stride elements from token to token (multiples of 8).  Sequence b has the
- * tokens cu_seqlens[b] to cu_seqlens[b + 1] (null: token b alone, total == batch) and puts them at positions[b] and on (null: 0).
+ * tokens cu_seqlens[b] to cu_seqlens[b + 1] (null: token b alone, total == batch) and puts them at positions[b] and on (null: 0; negative: a
+ * sequence that is left out).
  * For each page, head and kind with new rows: a = their largest magnitude, NaN as infinity; the scale becomes max(a * (1 / top),
  * 2^-100), top = 127 or 448, and at least the scale before where rows of the sequence come in front of the new ones in the page; their codes are then
  * rounded again from code * (scale before / scale).  A new code is x * (1 / scale), rounded to nearest even, or 0 under an infinite scale. */

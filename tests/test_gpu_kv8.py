@@ -147,6 +147,36 @@ def test_append_leaves_bad_pages_alone(fa):
         _same(got, want)
 
 
+@pytest.mark.parametrize("packed", [False, True])
+def test_padded_batches(fa, packed):
+    """Sequences with a negative position write nothing and report nothing; with a length of 0 they get zeros and add no weights."""
+    H, D, B = 2, 64, 5
+    state = kc.cache(8, H, D, torch.int8, 16)
+    table = torch.full((B, 2), -1, dtype=torch.int32)
+    table[1], table[3] = _ints([4, 2]), _ints([7, 0])
+    lens = [0, 20, 0, 17, 0]
+    g = torch.Generator().manual_seed(17)
+    cu = _ints([0, 3, 7, 12, 14, 15]) if packed else None
+    k, v = (torch.randn(15, H, D, generator=g).half() if packed else torch.randn(B, H, 1, D, generator=g).half() for _ in range(2))
+    pos = _ints([-1, 16 if packed else 19, -7, 15 if packed else 16, -2147483648])
+    dev, ref = [t.cuda() for t in state], [t.clone() for t in state]
+    fa.append_paged_kv8(k.cuda(), v.cuda(), *dev, table.cuda(), pos.cuda(), 2, cu_seqlens=None if cu is None else cu.cuda())
+    flat = lambda t: t.reshape(-1, H, D)
+    for b in (1, 3):
+        rows = slice(int(cu[b]), int(cu[b + 1])) if packed else slice(b, b + 1)
+        n = rows.stop - rows.start
+        orc.append(flat(k)[rows], flat(v)[rows], *ref, table[b: b + 1], pos[b: b + 1], _ints([0, n]))
+    for got, want in zip(dev, ref):
+        _same(got, want)
+    q, mass = torch.randn(B, 4, 1, D, generator=g).half(), torch.zeros(B, H, 32)
+    sums = mass.cuda()
+    out = fa.forward_paged_decode_gqa_kv8(q.cuda(), *dev, table.cuda(), _ints(lens).cuda(), 2, mass=sums)
+    want, size = orc.decode(q, *ref, table, lens)
+    bound, _ = kc.decode_bound(q, ref[0], ref[2], want, size, torch.float16, 0.0)
+    assert bool(((out.cpu().double() - want).abs() <= bound).all())
+    assert all(bool((out[b] == 0).all()) and bool((sums[b] == 0).all()) for b in (0, 2, 4))
+
+
 # ---- decode --------------------------------------------------------------------------------------------------------
 def _decode_case(fa, codes, dtype, H, G, D, T, lens, seed, softcap=0.0, mass=False, q_scale=1.0):
     pages = sum((max(0, n) + 15) // 16 for n in lens) + 3
@@ -488,6 +518,36 @@ def test_calls_on_another_stream_and_in_a_graph(fa):
                 assert torch.equal(kc.bits(a), kc.bits(b))
         for s in sets:
             s["lens"].add_(1); s["pos"].add_(1)
+
+
+def test_calls_on_two_streams_at_once(fa):
+    """Eager calls of two streams beside each other, each with a cache of its own, give what they give alone."""
+    lens = [2000, 40, 700, 1]
+    table, rest = kc.tables(lens, 400, 120)
+    new = _ints([rest[i * 8: i * 8 + 8] for i in range(4)]).cuda()
+    bt, n = table.cuda(), _ints(lens).cuda()
+    g = torch.Generator().manual_seed(121)
+    sets = [dict(dev=[t.cuda() for t in kc.cache(400, 2, 128, c, 122)], q=torch.randn(4, 8, 1, 128, generator=g).half().cuda(),
+                 k=torch.randn(4, 2, 1, 128, generator=g).half().cuda(), s=torch.cuda.Stream()) for c in CODES]
+
+    def run(s):
+        dev, mass = [t.clone() for t in s["dev"]], torch.zeros(4, 2, table.size(1) * 16).cuda()
+        for _ in range(5):
+            fa.append_paged_kv8(s["k"], s["k"], *dev, bt, n - 1, bt.size(1))
+            out = fa.forward_paged_decode_gqa_kv8(s["q"], *dev, bt, n, bt.size(1), mass=mass)
+            kept, _, _ = fa.evict_paged_kv8(mass, *dev, bt, n, bt.size(1), new, 128, 2, 8)
+        return dev + [mass, out, kept]
+
+    alone = [[kc.bits(t).cpu() for t in run(s)] for s in sets]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        both = []
+        for s in sets:
+            with torch.cuda.stream(s["s"]):
+                both.append(run(s))
+        torch.cuda.synchronize()
+        for got, want in zip(both, alone):
+            assert all(torch.equal(kc.bits(a).cpu(), b) for a, b in zip(got, want))
 
 
 FIRST_CALL_IN_A_GRAPH = """
