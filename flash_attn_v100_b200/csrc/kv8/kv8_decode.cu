@@ -14,7 +14,7 @@
 // The pages of all sequences and heads are cut evenly over the warps; where there are fewer segments than half the CTAs each is cut into equal
 // parts, at least kLeastPart pages, that the warps of a CTA share.  Parts of a cut segment go through global memory to a second launch, which, like the
 // first, is on its way before the launch in front of it has ended.
-// Measured, int8, 32 heads on 8 of 128: 64 sequences of 512 to 8192 tokens 110.8 us for 573 MB (5.2 TB/s), one of 131071 (e4m3) 51.3 us for 269 MB; four of up to
+// Measured, int8, 32 heads on 8 of 128: 64 sequences of 512 to 8192 tokens 110.8 us for 573 MB (5.2 TB/s), one of 131071 (e4m3) 51.0 us for 269 MB; four of up to
 // 101 tokens 5.7 us.  Two CTAs of four warps an SM, 16 KB of ring each: with three the first takes as long, the second 57 us (bytes on their way are enough
 // with eight warps, and more wait longer for theirs).  Of the first case 4 us pass before the memory is busy and 5 behind the last code; between them it
 // delivers 7.3 TB/s until the first SMs are through, and the last are a sixth later: some get their bytes slower than others.  Looked at and left: loads
@@ -236,8 +236,9 @@ __device__ __forceinline__ uint2 lds8(uint32_t at) {
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(at));
   return r;
 }
-__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+// Codes are read once: the hint lets what is read again, scores and parts, stay in L2 (a decode with sums 73.5 -> 71.2 us, others 1 to 2 %).
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "l"(policy) : "memory");
 }
 
 template <int D, int NT, bool E4M3>
@@ -325,6 +326,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
       asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint16_t*>(a.q) + q0 + lane * 64));
   };
   // Where a lane's pieces of rows go: the places repeat after kKinds copies, 512 bytes each.
+  const uint64_t policy = l2_policy_evict_first();
   constexpr int kKinds = D == 256 ? 4 : 2;
   uint32_t key_to[kKinds], value_to[kKinds];
 #pragma unroll
@@ -334,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
   }
   const auto copy_page = [&](const uint32_t (&to)[kKinds], int slot, int u, const uint8_t* from) {
 #pragma unroll
-    for (int c = 0; c < kCopies; ++c) copy16(to[c % kKinds] + slot * (2 * kTile * kPageBytes) + u * kPageBytes + c / kKinds * (kKinds * 512), from + c * 512);
+    for (int c = 0; c < kCopies; ++c) copy16(to[c % kKinds] + slot * (2 * kTile * kPageBytes) + u * kPageBytes + c / kKinds * (kKinds * 512), from + c * 512, policy);
   };
   const auto copy_keys = [&](int slot) {
     if (f_i < f.steps) {
