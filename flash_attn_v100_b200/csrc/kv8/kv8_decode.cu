@@ -475,6 +475,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
       l[n][0] = l[n][1] = 0.f;
     }
 
+    int spoiled = 0;                            // bit 2n + c: the row has seen a page whose V scale is not finite
     for (int i = 0; i < x.steps; ++i) {
       const int base = p0 + (turn + share * i) * kTile;
       cp_async_wait<2 * kSlots - 1>();
@@ -485,6 +486,14 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
         asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(ks[u]), "=f"(vs[u]) : "r"(scales_at + (at_slot * kTile + u) * 8));
         if (!(fabsf(ks[u]) <= 3.4028235e38f)) ks[u] = CUDART_NAN_F;      // a scale that is not finite spoils what sees the page, whatever the codes
         if (base + u >= p1) vs[u] = 0.f;
+        // So does V's, but 0 times it would also spoil what does not see the page: the rows that do are marked, and the page adds nothing.
+        if (!(fabsf(vs[u]) <= 3.4028235e38f)) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) spoiled |= (base + u) * kPage < limit[n][c] ? 1 << (n * 2 + c) : 0;
+          vs[u] = 0.f;
+        }
       }
       // ---- S^T = K Q^T
       float s[kTile][NT][4];
@@ -648,6 +657,15 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
       at_slot = at_slot + 1 == kSlots ? 0 : at_slot + 1;
     }
 
+    if (spoiled) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (spoiled >> (n * 2 + (e & 1)) & 1) o[n][k][e] = CUDART_NAN_F;
+    }
     Piece next;
     if (at < end) {                             // the next piece's rows come while this one's go out
       next = locate(at);

@@ -1,6 +1,6 @@
 """Operators on a paged cache in 8 bits (include/fa_b200_kv8.h): what writes it, what reads it and what makes it shorter.
 
-The cache keeps 16 tokens a page: k_cache and v_cache [pages, H_KV, 16, D], int8 (codes -127..127) or float8_e4m3fn, and kv_scale [pages, H_KV, 2]
+The cache keeps 16 tokens a page: k_cache and v_cache [pages, H_KV, 16, D], int8 (codes -127..127) or float8_e4m3fn (none of them NaN), and kv_scale [pages, H_KV, 2]
 fp32 with a scale for each page, head and kind (0: keys, 1: values), up to 2^60; a code stands for code * scale.  D is 64, 128 or 256.  block_table [B, *] int32
 with row stride `max_num_blocks` holds a sequence's pages in order, as in `forward_paged_decode_gqa_fp16`.  q, k, v are float16 or bfloat16.
 
@@ -134,8 +134,8 @@ def _check_mass(mass, mass_index, batch, c, like):
 def forward_paged_decode_gqa_kv8(q, k_cache, v_cache, kv_scale, block_table, seq_lens, max_num_blocks, softcap=0.0, mass=None, mass_index=None):
     """Attention of the newest T tokens of each sequence on a paged 8-bit cache.
 
-    q [B,H_Q,T,D], seq_lens [B] int32 (the T tokens counted in) -> new [B,H_Q,T,D].  Token t sees the keys before seq_len - T + t + 1; one that
-    sees none gets zeros.  With softcap > 0 a score x becomes softcap * tanh(x / softcap).  `mass` [rows,H_KV,tokens] fp32: what every key
+    q [B,H_Q,T,D], seq_lens [B] int32 (the T tokens counted in) -> new [B,H_Q,T,D].  Token t sees the keys before seq_len - T + t + 1 and is what those
+    make it, whatever the scales of pages behind them; one that sees none gets zeros.  With softcap > 0 a score x becomes softcap * tanh(x / softcap).  `mass` [rows,H_KV,tokens] fp32: what every key
     is given by the softmax, summed over the query heads of its KV head and the T tokens, is added in place to row mass_index[b] (None: b); the
     rows of a call must be different ones.  It takes 4 bytes of scratch for every query row and token that a block_table row has room for."""
     done = _native("kv8_decode", q, k_cache, v_cache, kv_scale, block_table, seq_lens, max_num_blocks, softcap, mass, mass_index)

@@ -1,9 +1,9 @@
 /* C ABI of the operators on a paged cache in 8 bits (libfa_b200_kv8.so, sm_100a): what writes it, what reads it, what makes it shorter.
  *
  * The cache keeps 16 tokens a page: codes [pages, heads, 16, dim] for keys and for values and a scale for each page, head and kind,
- * [pages, heads, 2] fp32 (0: keys, 1: values), from 0 to 2^60.  A code stands for code * scale; codes are int8 in -127..127 or e4m3.  dim is
- * 64, 128 or 256.  table [batch, *] int32 with row stride `width` holds a sequence's pages in order; of a row the first `max_pages`
- * entries are looked at, and a sequence has at most 16 * max_pages tokens.
+ * [pages, heads, 2] fp32 (0: keys, 1: values), from 0 to 2^60.  A code stands for code * scale; codes are int8 in -127..127 or e4m3, none of them
+ * NaN (what spoils a page is an infinite scale).  dim is 64, 128 or 256.  table [batch, *] int32 with row stride `width` holds a sequence's pages
+ * in order; of a row the first `max_pages` entries are looked at, and a sequence has at most 16 * max_pages tokens.
  *
  * Conventions: device pointers on the current device, 16-byte aligned where tensors of 8 or 16 bits are meant; every call is asynchronous
  * on `stream` (a cudaStream_t); nothing is allocated.  Return value: 0, or a negative code with a text in fak_last_error().  A page
@@ -48,7 +48,7 @@ int fak_append_paged(const FakCache* cache, const void* k, const void* v, int64_
                      const int32_t* cu_seqlens, int batch, int64_t total, void* stream);
 
 /* Attention of the `tokens` newest tokens of each sequence, q and out [batch, q_heads, tokens, dim]; lens [batch] counts them in.  Token t of
- * a sequence sees the keys before lens - tokens + t + 1; a row that sees none gives zeros.  Scores (q . k) / sqrt(dim), with softcap (0, or
+ * a sequence sees the keys before lens - tokens + t + 1, and no page behind those reaches it; a row that sees none gives zeros.  Scores (q . k) / sqrt(dim), with softcap (0, or
  * from 1e-30 to 1e30) softcap * tanh(score / softcap).  mass [mass_rows, heads, mass_cap] fp32, where given: every key's weights, summed over the rows of its head, are added to row
  * mass_index[b] (null: b), which must be another one for each b.  The workspace (16-byte aligned) has fak_decode_workspace bytes. */
 size_t fak_decode_workspace(const FakCache* cache, int batch, int q_heads, int tokens, int with_mass);

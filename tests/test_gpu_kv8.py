@@ -307,6 +307,35 @@ def test_decode_lengths_beyond_the_table_are_cut(fa):
     assert torch.equal(run(1000), run(32)) and bool((run(-3) == 0).all())
 
 
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("D,G", [(64, 2), (64, 5), (128, 4), (256, 1)])
+@pytest.mark.parametrize("how", ["keys", "values", "outside"])
+def test_decode_spoiled_pages_leave_earlier_tokens_alone(fa, codes, D, G, how):
+    """Of four new tokens those that do not see a page of an infinite scale, or one outside the cache, come out as if it were fine; those without keys stay zero."""
+    H, T, lens = 2, 4, [33, 65, 2, 17, 146]
+    seen_from = [3, 3, 2, 4, 2]                                   # the first new token that sees the last page (sequence 3: left fine)
+    table, rest = kc.tables(lens, 24, 130)
+    k8, v8, scale = kc.cache(24, H, D, codes, 131)
+    q = torch.randn(len(lens), H * G, T, D, generator=torch.Generator().manual_seed(132)).half().cuda()
+    args = lambda k, v, s, t: (q, k.cuda(), v.cuda(), s.cuda(), t.cuda(), _ints(lens).cuda(), t.size(1))
+    fine = fa.forward_paged_decode_gqa_kv8(*args(k8, v8, scale, table))
+    assert bool(fine.isfinite().all()) and bool((fine[2, :, :2] == 0).all())
+    for b in (0, 1, 2, 4):
+        at = (lens[b] - 1) // 16
+        if how == "outside":
+            table[b, at] = 24
+            continue
+        kind = 0 if how == "keys" else 1
+        scale[int(table[b, at]), :, kind] = math.inf
+        kc.bits((k8, v8)[kind])[int(table[b, at])] = 0
+    out = fa.forward_paged_decode_gqa_kv8(*args(k8, v8, scale, table))
+    for b, t in enumerate(seen_from):
+        assert torch.equal(out[b, :, :t], fine[b, :, :t]) and bool(out[b, :, t:].isnan().all())
+    if how == "outside":
+        with pytest.raises(RuntimeError, match="outside the cache"):
+            fa.check_async_errors()
+
+
 def test_caches_of_more_than_32_bits(fa):
     """Pages whose codes lie beyond 2^32 bytes."""
     H, D, lens = 8, 256, [50]
