@@ -40,7 +40,8 @@ struct DecodeArgs {
   const int* lens;
   int batch, rows, tokens;      // rows: query rows of a KV head, (heads of its group) x tokens
   bool bf16, capped;
-  float scale, cap, inv_cap;    // score scale, in base 2 without a cap; cap in base 2, 2 log2 e / cap
+  float scale;                  // of scores in base 2
+  float cap, inv_cap, cap_exp, near;      // cap of scores in base 2, 1 / cap, 2 log2 e / cap, cap / 4
   float* mass;
   const int* mass_index;
   int mass_rows, mass_cap;

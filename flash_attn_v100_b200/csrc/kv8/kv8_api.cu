@@ -155,9 +155,11 @@ int fak_decode_paged(const FakCache* cache, const void* q, void* out, const int3
   uint8_t* base = static_cast<uint8_t*>(workspace);
   const double log2e = 1.4426950408889634, root = 1.0 / sqrt((double)cache->dim);
   a.rows = rows; a.tokens = tokens; a.bf16 = dtype == FAK_BF16; a.capped = softcap > 0.f;
-  a.scale = (float)(a.capped ? root : root * log2e);
+  a.scale = (float)(root * log2e);
   a.cap = (float)(softcap * log2e);
-  a.inv_cap = a.capped ? (float)(2.0 * log2e / softcap) : 0.f;
+  a.inv_cap = a.capped ? (float)(1.0 / (softcap * log2e)) : 0.f;
+  a.cap_exp = a.capped ? (float)(2.0 / softcap) : 0.f;
+  a.near = 0.25f * a.cap;
   a.n_cta = d.n_cta; a.blocks = d.blocks; a.score_cols = d.score_cols;
   a.plan = reinterpret_cast<int*>(base + w.plan);
   a.part = reinterpret_cast<float*>(base + w.part);

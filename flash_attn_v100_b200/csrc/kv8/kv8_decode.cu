@@ -41,11 +41,17 @@ __device__ __forceinline__ float log2_of(float x) {
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// cap tanh(x inv_cap) = cap (1 - 2 / (e^(2 x inv_cap) + 1)), off by less than 2^-21 cap; inv_cap comes times 2 log2 e.
-__device__ __forceinline__ float capped(float x, float cap, float inv_cap) {
+// A score x in base 2 under its cap, both ways to 2^-19 of the result: from a quarter of the cap on cap tanh(x / cap) = cap (1 - 2 / (e^(2x / cap) + 1)), off by
+// less than 2^-21 cap, and below x (1 - u^2/3 + 2 u^4/15 - 17 u^6/315), u = x / cap, whose next term is 2^-21 of x.  (The first alone loses the scores
+// of large caps: 1 % of the weights at 1e5, all at 1e8.)
+__device__ __forceinline__ float capped_far(float x, const DecodeArgs& a) {
   float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(fast_exp2(x * inv_cap) + 1.f));
-  return fmaf(-2.f * cap, r, cap);
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(fast_exp2(x * a.cap_exp) + 1.f));
+  return fmaf(-2.f * a.cap, r, a.cap);
+}
+__device__ __forceinline__ float capped_near(float x, const DecodeArgs& a) {
+  const float u = x * a.inv_cap, u2 = u * u;
+  return fmaf(x * u2, fmaf(u2, fmaf(u2, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), x);
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -528,12 +534,31 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[u][n][e] *= factor[n][e & 1] * ks[u];
       if (a.capped) {
+        bool far = false;
 #pragma unroll
         for (int u = 0; u < kTile; ++u)
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[u][n][e] = capped(s[u][n][e], a.cap, a.inv_cap);
+            for (int e = 0; e < 4; ++e) far |= fabsf(s[u][n][e]) >= a.near;
+        if (__any_sync(0xffffffffu, far)) {
+#pragma unroll
+          for (int u = 0; u < kTile; ++u)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float x = s[u][n][e], y = capped_near(x, a), z = capped_far(x, a);
+                s[u][n][e] = fabsf(x) >= a.near ? z : y;
+              }
+        } else {
+#pragma unroll
+          for (int u = 0; u < kTile; ++u)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[u][n][e] = capped_near(s[u][n][e], a);
+        }
       }
       const bool masked = key0 + kTile * kPage > free_keys || base + kTile > p1;
       if (masked) {

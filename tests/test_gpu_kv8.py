@@ -336,6 +336,37 @@ def test_decode_spoiled_pages_leave_earlier_tokens_alone(fa, codes, D, G, how):
             fa.check_async_errors()
 
 
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("D,G", [(64, 4), (128, 9), (256, 4)])
+@pytest.mark.parametrize("softcap", [1e-30, 0.5, 30.0, 1e3, 1e5, 1e6, 1e30])
+def test_decode_caps_of_all_sizes(fa, codes, D, G, softcap):
+    """Up to the largest cap that is accepted, which leaves the scores as they are.
+
+    The cap's error goes by the score: 2^-19 of it, from a quarter of the cap on an error of 2^-21 of the cap, and a polynomial's 2^-20 below."""
+    H, T, lens = 2, 2, LENS
+    table, _ = kc.tables(lens, 40, 133)
+    k8, v8, scale = kc.cache(40, H, D, codes, 134)
+    g = torch.Generator().manual_seed(135)
+    q = (torch.randn(len(lens), H * G, T, D, generator=g) * 2).half()
+    sums = torch.zeros(len(lens), H, table.size(1) * 16)
+    dev, sums64 = sums.cuda(), sums.double()
+    out = fa.forward_paged_decode_gqa_kv8(q.cuda(), k8.cuda(), v8.cuda(), scale.cuda(), table.cuda(), _ints(lens).cuda(), table.size(1), softcap=softcap, mass=dev)
+    ref, size = orc.decode(q, k8, v8, scale, table, lens, softcap, sums64)
+    _, delta = kc.decode_bound(q, k8, scale, ref, size, torch.float16, 0.0)
+    most = 0.0                                                    # the largest score of all
+    for b, n in enumerate(lens):
+        for h in range(H):
+            rows = orc.rows_of(k8, scale, 0, table[b], h, n)
+            if n:
+                most = max(most, float((q[b, h * G: h * G + G].double().reshape(-1, D) @ rows.T).abs().max()) / math.sqrt(D))
+    delta += min(most, softcap) * 2.0 ** -19
+    assert delta < 2.0 ** -7
+    bound = ref.abs() * kc.half_step(torch.float16) + size * (2.0 ** -11 + 2 * delta) + float(size.max()) * 2.0 ** -20
+    off = (out.cpu().double() - ref).abs()
+    assert bool((off <= bound).all()), (off / bound).max().item()
+    assert bool(((dev.cpu().double() - sums64).abs() <= sums64 * (2 * delta + 2.0 ** -18)).all())
+
+
 def test_caches_of_more_than_32_bits(fa):
     """Pages whose codes lie beyond 2^32 bytes."""
     H, D, lens = 8, 256, [50]
