@@ -8,9 +8,9 @@
 // A warp copies pages to a ring of its own in shared memory (cp.async, 16 bytes a lane, the pieces of a row placed so that the reads meet no bank twice) and
 // runs ahead of its own reads from one piece into the next.  A lane's 16 bytes of a key row are four steps of the (permuted) contraction, and its 16
 // bytes of four tokens' values the rows of eight tiles of O^T.  They become fp16 in registers, exactly.
-// K's scale multiplies the finished scores.  V's scale goes into the exponent: with m the running maximum of s + log2 vs the weight that meets the
-// codes is 2^(s - m) vs <= 1, so fp16 keeps 11 bits of the products that matter whatever the pages' scales are; the sum of weights
-// takes 2^(s - m) in fp32.
+// K's scale multiplies the finished scores.  V's scale goes into the exponent: with m the running maximum of s + log2 vs, less 15, the weight that meets the
+// codes is 2^(s - m) vs <= 2^15, so fp16 keeps 11 bits of the products down to 2^-29 of the largest whatever the pages' scales are (with 1 as the largest weight
+// all below 2^-25 were lost, of many tokens behind a strong one a visible part); the sum of weights takes 2^(s - m) in fp32.
 // The pages of all sequences and heads are cut evenly over the warps; where there are fewer segments than half the CTAs each is cut into equal
 // parts, at least kLeastPart pages, that the warps of a CTA share.  Parts of a cut segment go through global memory to a second launch, which, like the
 // first, is on its way before the launch in front of it has ended.
@@ -34,7 +34,7 @@ namespace {
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kLeastPart = 8;
 constexpr int kOpening = 4;
-
+constexpr float kTop = 15.f;      // a weight times V's scale is at most 2 to this: fp16 ends at 2^16
 
 __device__ __forceinline__ float log2_of(float x) {
   float y;
@@ -585,12 +585,12 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
                 if (n * 8 + 2 * t < cols)
                   *reinterpret_cast<float2*>(to + (u * kPage + g + half * 8) * cols + n * 8 + 2 * t) = make_float2(s[u][n][half * 2], s[u][n][half * 2 + 1]);
       }
-      // ---- running maximum of s + log2 vs
+      // ---- running maximum of s + log2 vs, less 15
       uint32_t pf[kTile][NT][2];
       bool moved = false;
       float top[NT][2], lv[kTile];
 #pragma unroll
-      for (int u = 0; u < kTile; ++u) lv[u] = fminf(fmaxf(log2_of(vs[u]), -60.f), 60.f);
+      for (int u = 0; u < kTile; ++u) lv[u] = fminf(fmaxf(log2_of(vs[u]), -60.f), 60.f) - kTop;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -632,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
         const float ref[2] = {m[n][0] == -CUDART_INF_F ? 0.f : m[n][0], m[n][1] == -CUDART_INF_F ? 0.f : m[n][1]};
 #pragma unroll
         for (int u = 0; u < kTile; ++u) {
-          float p[4];                             // (at most 2^60, and times vs at most 1)
+          float p[4];                             // (at most 2^75, and times vs at most 2^15)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             p[e] = fast_exp2(s[u][n][e] - ref[e & 1]);

@@ -367,6 +367,35 @@ def test_decode_caps_of_all_sizes(fa, codes, D, G, softcap):
     assert bool(((dev.cpu().double() - sums64).abs() <= sums64 * (2 * delta + 2.0 ** -18)).all())
 
 
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_decode_tails_behind_a_strong_token(fa, codes, D):
+    """Weights far below the largest add to the result as they add to the sum: one token takes nearly all of the weight and has no value, the others have 1000.
+
+    Weights times V's scale are fp16 with 2^14 at least for the largest: 2^-28 of that is still a normal number, off by 2^-11."""
+    B, n = 2400, 200                                              # (so many that a warp has whole sequences; they share their pages)
+    top = orc.TOP[codes]
+    k8, v8 = (torch.zeros(13, 1, 16, D) for _ in range(2))
+    k8[0, 0, 0, 0] = top
+    v8[:] = top
+    v8[0, 0, 0] = 0
+    scale = torch.empty(13, 1, 2)
+    scale[..., 0], scale[..., 1] = 1 / top, 1000 / top
+    k8, v8 = k8.to(codes), v8.to(codes)
+    below = torch.tensor([18.0, 22.0, 25.5, 28.0])[torch.arange(B) % 4]
+    q = torch.zeros(B, 1, 1, D)
+    q[:, 0, 0, 0] = below * math.log(2) * math.sqrt(D)
+    q = q.half()
+    table = torch.arange(13).int()[None].expand(B, -1).contiguous()
+    out = fa.forward_paged_decode_gqa_kv8(q.cuda(), k8.cuda(), v8.cuda(), scale.cuda(), table.cuda(), torch.full((B,), n).int().cuda(), 13)
+    s = q[:, 0, 0, :1].double() * float(scale[0, 0, 0]) * top / math.sqrt(D)
+    tails = (n - 1) * torch.exp(-s)
+    ref = 1000.0 * tails / (1 + tails)
+    delta = float(s.max()) * 2.0 ** -20 + 2.0 ** -18              # (one product; the factors' and the exponential's roundings)
+    off = (out[:, 0, 0].cpu().double() - ref).abs()
+    assert bool((off <= ref * (kc.half_step(torch.float16) + 2.0 ** -11 + 2 * delta)).all()), (off / ref).max().item()
+
+
 def test_caches_of_more_than_32_bits(fa):
     """Pages whose codes lie beyond 2^32 bytes."""
     H, D, lens = 8, 256, [50]
