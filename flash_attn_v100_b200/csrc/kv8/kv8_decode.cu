@@ -8,9 +8,10 @@
 // A warp copies pages to a ring of its own in shared memory (cp.async, 16 bytes a lane, the pieces of a row placed so that the reads meet no bank twice) and
 // runs ahead of its own reads from one piece into the next.  A lane's 16 bytes of a key row are four steps of the (permuted) contraction, and its 16
 // bytes of four tokens' values the rows of eight tiles of O^T.  They become fp16 in registers, exactly.
-// K's scale multiplies the finished scores.  V's scale goes into the exponent: with m the running maximum of s + log2 vs, less 15, the weight that meets the
-// codes is 2^(s - m) vs <= 2^15, so fp16 keeps 11 bits of the products down to 2^-29 of the largest whatever the pages' scales are (with 1 as the largest weight
-// all below 2^-25 were lost, of many tokens behind a strong one a visible part); the sum of weights takes 2^(s - m) in fp32.
+// K's scale multiplies the finished scores.  V's scale goes into the exponent: with m the running maximum of s + log2 vs, less 25, the weight that meets the
+// codes is 2^(s - m) vs / 2^10 <= 2^15, so fp16 keeps 11 bits of the products down to 2^-29 of the largest (with 1 as the largest weight all below 2^-25 were
+// lost, of many tokens behind a strong one a visible part); the sum of weights takes 2^(s - m) in fp32, which has room for every scale that an append makes:
+// it is 2^-96 at 2^121 and at most 2^100 at 2^-100, where log2 vs counts as -75 and the weights reach 2^-10.
 // The pages of all sequences and heads are cut evenly over the warps; where there are fewer segments than half the CTAs each is cut into equal
 // parts, at least kLeastPart pages, that the warps of a CTA share.  Parts of a cut segment go through global memory to a second launch, which, like the
 // first, is on its way before the launch in front of it has ended.
@@ -34,7 +35,8 @@ namespace {
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kLeastPart = 8;
 constexpr int kOpening = 4;
-constexpr float kTop = 15.f;      // a weight times V's scale is at most 2 to this: fp16 ends at 2^16
+constexpr float kUnit = 1024.f, kTop = 25.f;      // a weight times V's scale is at most kUnit * 2^15: fp16 ends at 2^16
+constexpr float kLeastLog = -75.f;                // of V's scale
 
 __device__ __forceinline__ float log2_of(float x) {
   float y;
@@ -53,6 +55,8 @@ __device__ __forceinline__ float capped_near(float x, const DecodeArgs& a) {
   const float u = x * a.inv_cap, u2 = u * u;
   return fmaf(x * u2, fmaf(u2, fmaf(u2, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), x);
 }
+// The root of 2^(m - top): a sum of weights goes from m to top in two steps, as it may be large where the factor is below fp32's range.
+__device__ __forceinline__ float half_step(float m, float top) { return fast_exp2(0.5f * (m - top)); }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -585,12 +589,15 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
                 if (n * 8 + 2 * t < cols)
                   *reinterpret_cast<float2*>(to + (u * kPage + g + half * 8) * cols + n * 8 + 2 * t) = make_float2(s[u][n][half * 2], s[u][n][half * 2 + 1]);
       }
-      // ---- running maximum of s + log2 vs, less 15
+      // ---- running maximum of s + log2 vs, less 25
       uint32_t pf[kTile][NT][2];
       bool moved = false;
       float top[NT][2], lv[kTile];
 #pragma unroll
-      for (int u = 0; u < kTile; ++u) lv[u] = fminf(fmaxf(log2_of(vs[u]), -60.f), 60.f) - kTop;
+      for (int u = 0; u < kTile; ++u) {
+        lv[u] = fmaxf(log2_of(vs[u]), kLeastLog) - kTop;
+        vs[u] *= 1.f / kUnit;
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -617,9 +624,10 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             top[n][c] = fmaxf(m[n][c], top[n][c]);
-            shrink[c] = top[n][c] == -CUDART_INF_F ? 1.f : fast_exp2(m[n][c] - top[n][c]);
+            const float half = top[n][c] == -CUDART_INF_F ? 1.f : half_step(m[n][c], top[n][c]);
             m[n][c] = top[n][c];
-            l[n][c] *= shrink[c];
+            l[n][c] = l[n][c] * half * half;
+            shrink[c] = half * half;
           }
 #pragma unroll
           for (int k = 0; k < kSteps; ++k)
@@ -632,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
         const float ref[2] = {m[n][0] == -CUDART_INF_F ? 0.f : m[n][0], m[n][1] == -CUDART_INF_F ? 0.f : m[n][1]};
 #pragma unroll
         for (int u = 0; u < kTile; ++u) {
-          float p[4];                             // (at most 2^75, and times vs at most 2^15)
+          float p[4];                             // (at most 2^100, and times vs at most 2^15)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             p[e] = fast_exp2(s[u][n][e] - ref[e & 1]);
@@ -712,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
           const int r = n * 8 + 2 * t + c;
           if (r >= rows) continue;
           if (whole) {
-            const float inv = l[n][c] == 0.f ? 0.f : 1.f / l[n][c];
+            const float inv = l[n][c] == 0.f ? 0.f : kUnit / l[n][c];
             uint16_t* to = static_cast<uint16_t*>(a.out) + (head * a.rows + r0 + r) * D + g * (D / 8);
 #pragma unroll
             for (int k = 0; k < kSteps; k += 4) {
@@ -758,13 +766,13 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = fast_exp2(sm_ml(w)[r * 2] - ref);
-        sum += sm_ml(w)[r * 2 + 1] * f;
+        const float half = half_step(sm_ml(w)[r * 2], ref), f = half * half;
+        sum += sm_ml(w)[r * 2 + 1] * half * half;
         const float4 x = *reinterpret_cast<const float4*>(sm_o(w) + r * (D + 4) + d);
         acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
       }
       if (whole) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const float inv = sum == 0.f ? 0.f : kUnit / sum;
         uint2 packed = make_uint2(pack_out16x2(acc.x * inv, acc.y * inv, a.bf16), pack_out16x2(acc.z * inv, acc.w * inv, a.bf16));
         *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (head * a.rows + r0 + r) * D + d) = packed;
       } else {
@@ -837,8 +845,8 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const DecodeArgs a, int
   for (int i = warp; i < x.n; i += W) {
     const int64_t slot = x.slot(i) * row_block + r;
     const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + slot * 2);
-    const float f = fast_exp2(ml.x - ref);
-    sum += ml.y * f;
+    const float half = half_step(ml.x, ref), f = half * half;
+    sum += ml.y * half * half;
     const float4* p = reinterpret_cast<const float4*>(a.part + slot * D);
 #pragma unroll
     for (int e = 0; e < kEach; ++e)
@@ -865,7 +873,7 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const DecodeArgs a, int
       sum += sm[w][1];
     }
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const float inv = sum == 0.f ? 0.f : kUnit / sum;
   uint16_t* out = static_cast<uint16_t*>(a.out) + (head * a.rows + row) * D;
 #pragma unroll
   for (int e = 0; e < kEach; ++e)

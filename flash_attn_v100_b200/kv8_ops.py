@@ -1,7 +1,7 @@
 """Operators on a paged cache in 8 bits (include/fa_b200_kv8.h): what writes it, what reads it and what makes it shorter.
 
 The cache keeps 16 tokens a page: k_cache and v_cache [pages, H_KV, 16, D], int8 (codes -127..127) or float8_e4m3fn (none of them NaN), and kv_scale [pages, H_KV, 2]
-fp32 with a scale for each page, head and kind (0: keys, 1: values), up to 2^60; a code stands for code * scale.  D is 64, 128 or 256.  block_table [B, *] int32
+fp32 with a scale for each page, head and kind (0: keys, 1: values), from 0 up; a code stands for code * scale.  D is 64, 128 or 256.  block_table [B, *] int32
 with row stride `max_num_blocks` holds a sequence's pages in order, as in `forward_paged_decode_gqa_fp16`.  q, k, v are float16 or bfloat16.
 
 Calls go to the current stream of the tensors' device and can be captured in CUDA graphs; there is no CPU path.  A page outside the

@@ -1,7 +1,7 @@
 /* C ABI of the operators on a paged cache in 8 bits (libfa_b200_kv8.so, sm_100a): what writes it, what reads it, what makes it shorter.
  *
  * The cache keeps 16 tokens a page: codes [pages, heads, 16, dim] for keys and for values and a scale for each page, head and kind,
- * [pages, heads, 2] fp32 (0: keys, 1: values), from 0 to 2^60.  A code stands for code * scale; codes are int8 in -127..127 or e4m3, none of them
+ * [pages, heads, 2] fp32 (0: keys, 1: values), from 0 up.  A code stands for code * scale; codes are int8 in -127..127 or e4m3, none of them
  * NaN (what spoils a page is an infinite scale).  dim is 64, 128 or 256.  table [batch, *] int32 with row stride `width` holds a sequence's pages
  * in order; of a row the first `max_pages` entries are looked at, and a sequence has at most 16 * max_pages tokens.
  *

@@ -396,6 +396,74 @@ def test_decode_tails_behind_a_strong_token(fa, codes, D):
     assert bool((off <= ref * (kc.half_step(torch.float16) + 2.0 ** -11 + 2 * delta)).all()), (off / ref).max().item()
 
 
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("lens", [[100, 64, 17], [3000], [90] * 320], ids=["whole", "parts", "even"])
+@pytest.mark.parametrize("power", [-92, -60, 60, 112])
+def test_decode_of_values_near_the_ends_of_bfloat16(fa, codes, lens, power):
+    """Values around 2^power, as an append stores them."""
+    H, G, D = 1, 4, 64
+    pages = sum((n + 15) // 16 for n in lens)
+    table, _ = kc.tables(lens, pages, 136)
+    state = kc.cache(pages, H, D, codes, 137)
+    dev, ref = [t.cuda() for t in state], [t.clone() for t in state]
+    g = torch.Generator().manual_seed(138)
+    k, v = torch.randn(sum(lens), H, D, generator=g).bfloat16(), (torch.randn(sum(lens), H, D, generator=g) * 2.0 ** power).bfloat16()
+    cu = _ints([0] + torch.tensor(lens).cumsum(0).tolist())
+    fa.append_paged_kv8(k.cuda(), v.cuda(), *dev, table.cuda(), None, table.size(1), cu_seqlens=cu.cuda())
+    orc.append(k, v, *ref, table, None, cu)
+    q = torch.randn(len(lens), H * G, 1, D, generator=g).bfloat16()
+    sums = torch.zeros(len(lens), H, table.size(1) * 16)
+    got, sums64 = sums.cuda(), sums.double()
+    out = fa.forward_paged_decode_gqa_kv8(q.cuda(), *dev, table.cuda(), _ints(lens).cuda(), table.size(1), mass=got)
+    want, size = orc.decode(q, *ref, table, lens, mass=sums64)
+    bound, delta = kc.decode_bound(q, ref[0], ref[2], want, size, torch.bfloat16, 0.0)
+    off = (out.cpu().double() - want).abs()
+    assert bool((off <= bound).all()), (off / bound).max().item()
+    assert bool(((got.cpu().double() - sums64).abs() <= sums64 * (2 * delta + 2.0 ** -18)).all())
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("lens", [[128, 100], [3000], [192] * 320], ids=["whole", "parts", "even"])
+@pytest.mark.parametrize("order", ["rising", "falling", "zeros first", "zeros last", "heavy and small"])
+def test_decode_of_pages_whose_scales_are_far_apart(fa, codes, lens, order):
+    """Scales that rise or fall from page to page, pages of zero rows (2^-100, as an append makes them) beside others, and small values that take the weight from large ones."""
+    H, G, D = 1, 4, 64
+    pages = sum((n + 15) // 16 for n in lens)
+    table, _ = kc.tables(lens, pages, 139)
+    k8, v8, scale = kc.cache(pages, H, D, codes, 140)
+    g = torch.Generator().manual_seed(141)
+    q = torch.randn(len(lens), H * G, 1, D, generator=g).bfloat16()
+    for b, n in enumerate(lens):
+        own = table[b, : (n + 15) // 16].long()
+        i = torch.arange(own.numel()).float() * (180.0 / own.numel())
+        if order == "rising":
+            scale[own, 0, 1] = torch.exp2(i - 90)
+        elif order == "falling":
+            scale[own, 0, 1] = torch.exp2(90 - i)
+        elif order.startswith("zeros"):
+            zero = own[:3] if order == "zeros first" else own[-3:]
+            scale[zero, 0, 1] = 2.0 ** -100
+            kc.bits(v8)[zero] = 0
+        else:                                                     # every other page: 2^40 larger values, and scores 50 lower in base 2
+            kc.bits(k8)[own[::2]] = 0
+            kc.bits(k8)[own, :, :, 0] = 0x7F if codes == torch.int8 else 0x7E      # the largest code
+            scale[own, 0, 0] = 1 / orc.TOP[codes]
+            kc.bits(k8)[own[::2], :, :, 0] = 0
+            scale[own[::2], 0, 1] = 2.0 ** 40
+            scale[own[1::2], 0, 1] = 1.0
+    if order == "heavy and small":
+        q *= 0.125
+        q[..., 0] = 50 * math.log(2) * math.sqrt(D)
+    sums = torch.zeros(len(lens), H, table.size(1) * 16)
+    got, sums64 = sums.cuda(), sums.double()
+    out = fa.forward_paged_decode_gqa_kv8(q.cuda(), k8.cuda(), v8.cuda(), scale.cuda(), table.cuda(), _ints(lens).cuda(), table.size(1), mass=got)
+    want, size = orc.decode(q, k8, v8, scale, table, lens, mass=sums64)
+    bound, delta = kc.decode_bound(q, k8, scale, want, size, torch.bfloat16, 0.0)
+    off = (out.cpu().double() - want).abs()
+    assert bool((off <= bound).all()), (off / bound).max().item()
+    assert bool(((got.cpu().double() - sums64).abs() <= sums64 * (2 * delta + 2.0 ** -18)).all())
+
+
 def test_caches_of_more_than_32_bits(fa):
     """Pages whose codes lie beyond 2^32 bytes."""
     H, D, lens = 8, 256, [50]
