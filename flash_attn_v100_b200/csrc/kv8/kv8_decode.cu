@@ -451,9 +451,11 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
         most = max(most & 0xffffu, most >> 16);
         most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const int e = min(max((int)(most >> 7) - 127, -126), 126);      // the largest magnitude's exponent
-        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-        up = __uint_as_float((uint32_t)(127 + e) << 23);
+        // The largest magnitude, of exponent e, goes to between 2^14 and 2^15: elements down to 2^-30 of it keep all their bits, smaller ones are off by at
+        // most 2^-39 of it.
+        const int e = min(max((int)(most >> 7) - 127, -112), 127);
+        const float down = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+        up = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
 #pragma unroll
         for (int i = 0; i < kSteps; ++i)
 #pragma unroll

@@ -464,6 +464,31 @@ def test_decode_of_pages_whose_scales_are_far_apart(fa, codes, lens, order):
     assert bool(((got.cpu().double() - sums64).abs() <= sums64 * (2 * delta + 2.0 ** -18)).all())
 
 
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("power", [-100, 0, 100])
+def test_decode_of_queries_with_one_large_element(fa, codes, D, power):
+    """Elements 2^22 below a bfloat16 row's largest keep their bits: the keys have nothing where the largest is, and the others decide the scores."""
+    H, G, lens = 2, 4, [100, 64]
+    table, _ = kc.tables(lens, 12, 142)
+    k8, v8, scale = kc.cache(12, H, D, codes, 143)
+    kc.bits(k8)[..., 5] = 0
+    scale[..., 0] *= 2.0 ** -power
+    small = (torch.randn(2, H * G, 1, D, generator=torch.Generator().manual_seed(144)) * 2.0 ** power).bfloat16()
+    small[..., 5] = 0
+    q = small.clone()
+    q[..., 5] = 1.5 * 2.0 ** (22 + power)
+    out = fa.forward_paged_decode_gqa_kv8(q.cuda(), k8.cuda(), v8.cuda(), scale.cuda(), table.cuda(), _ints(lens).cuda(), table.size(1))
+    ref, size = orc.decode(small, k8, v8, scale, table, lens)
+    _, delta = kc.decode_bound(small, k8, scale, ref, size, torch.bfloat16, 0.0)
+    # an element is off by at most 2^-39 of the largest (half of fp16's least step, under a largest of 2^14 or more): D of them, each with the largest code
+    delta += 1.5 * 2.0 ** (22 + power) * 2.0 ** -39 * D * orc.TOP[codes] * float(scale[..., 0].max()) / math.sqrt(D)
+    assert delta < 2.0 ** -8
+    bound = ref.abs() * kc.half_step(torch.bfloat16) + size * (2.0 ** -11 + 2 * delta) + float(size.max()) * 2.0 ** -20
+    off = (out.cpu().double() - ref).abs()
+    assert bool((off <= bound).all()), (off / bound).max().item()
+
+
 def test_caches_of_more_than_32_bits(fa):
     """Pages whose codes lie beyond 2^32 bytes."""
     H, D, lens = 8, 256, [50]
