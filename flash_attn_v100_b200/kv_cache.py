@@ -308,7 +308,10 @@ class PagedKVCache8(BlockManager):
 
     `codes` is torch.int8 or torch.float8_e4m3fn.  With `eviction` every layer keeps the sums of weights of each request's
     tokens, [max_batch, H_KV, tokens] in fp32, which `attend` adds to and `evict` goes by.  A request that was cut has
-    `get_cache_len` tokens in the cache and `position` tokens behind it: rotary angles go by the latter."""
+    `get_cache_len` tokens in the cache and `position` tokens behind it: rotary angles go by the latter.
+
+    Guessed tokens are appended and attended to together; `commit` takes how many of them stay, and the weights that the others gave are
+    taken back.  (Their rows are written over by the next tokens.  The scale that they asked of a block they share with tokens that stay is not taken back.)"""
 
     def __init__(self, num_blocks: int, num_layers: int, num_kv_heads: int, head_dim: int, max_batch: int, max_blocks_per_seq: int,
                  device="cuda", codes=torch.int8, enable_prefix_cache: bool = True, eviction: bool = True):
@@ -326,6 +329,8 @@ class PagedKVCache8(BlockManager):
         self.masses = [torch.zeros((max_batch, num_kv_heads, max_blocks_per_seq * BLOCK_SIZE), device=self.device)
                        for _ in range(num_layers)] if eviction else None
         self._positions: Dict[str, int] = {}                     # request -> tokens it has had
+        # request -> layer -> attentions of several tokens that are not committed: (place in the batch, the batch's sums before the first, q, softcap)
+        self._guessed: Dict[str, Dict[int, list]] = {}
 
     # ---- bookkeeping ----------------------------------------------------------------
     def allocate(self, request_id: str, num_tokens: int = 0, token_ids: Optional[Sequence[int]] = None) -> int:
@@ -336,12 +341,16 @@ class PagedKVCache8(BlockManager):
         return row
 
     def commit(self, request_id: str, num_new_tokens: int) -> None:
+        """Advance the token count by the appended tokens that stay.  Where `attend` has added the weights of more than those to the sums, they are
+        put back and those of the tokens that stay are added again."""
         super().commit(request_id, num_new_tokens)
         self._positions[request_id] += num_new_tokens
+        self._settle(request_id, num_new_tokens)
 
     def release(self, request_id: str) -> None:
         super().release(request_id)
         self._positions.pop(request_id, None)
+        self._guessed.pop(request_id, None)
 
     def position(self, request_id: str) -> int:
         """Tokens the request has had, evicted ones among them: the position of its next token."""
@@ -374,15 +383,41 @@ class PagedKVCache8(BlockManager):
 
     def attend(self, layer: int, request_ids: Sequence[str], q, softcap: float = 0.0, track: bool = True):
         """Attention of q [B, H_Q, T, D], each request's newest T tokens (appended, not committed yet); with `track` (and `eviction`)
-        their weights are added to the tokens' sums."""
+        their weights are added to the tokens' sums.  Of T > 1 tokens `commit` may keep fewer; a single one is taken to stay."""
         from . import kv8_ops
         table, lens = self.batch_view(request_ids, extra_tokens=q.size(2))
         mass = self.masses[layer] if track and self.masses is not None else None
-        rows = None
+        rows = before = None
         if mass is not None:
             rows = torch.tensor([self._row[r] for r in request_ids], dtype=torch.int32).to(self.device)
-        return kv8_ops.forward_paged_decode_gqa_kv8(q, self.k_pools[layer], self.v_pools[layer], self.scales[layer], table, lens,
-                                                    self.max_blocks_per_seq, softcap=softcap, mass=mass, mass_index=rows)
+            if request_ids and (q.size(2) > 1 or any(r in self._guessed for r in request_ids)):
+                before = mass[rows.long(), :, : max(self._tokens[r] for r in request_ids) + q.size(2)]
+        out = kv8_ops.forward_paged_decode_gqa_kv8(q, self.k_pools[layer], self.v_pools[layer], self.scales[layer], table, lens,
+                                                   self.max_blocks_per_seq, softcap=softcap, mass=mass, mass_index=rows)
+        if before is not None:
+            kept_q = q.clone()
+            for i, r in enumerate(request_ids):
+                calls = self._guessed.setdefault(r, {}).setdefault(layer, [])
+                calls.append((i, None if calls else before, kept_q, softcap))
+        return out
+
+    def _settle(self, request_id: str, kept: int) -> None:
+        """The sums of weights as if only the first `kept` (committed by now) of the tokens attended to since the last commit had been there."""
+        from . import kv8_ops
+        row, held = self._row[request_id], self._tokens[request_id] - kept
+        for layer, calls in self._guessed.pop(request_id, {}).items():
+            if all(q.size(2) <= kept for _, _, q, _ in calls):
+                continue
+            i, before, _, _ = calls[0]
+            self.masses[layer][row, :, : before.size(2)] = before[i]
+            index = torch.tensor([row], dtype=torch.int32).to(self.device)
+            for i, _, q, softcap in calls:
+                n = min(kept, q.size(2))
+                if n > 0:
+                    lens = torch.tensor([held + n], dtype=torch.int32).to(self.device)
+                    kv8_ops.forward_paged_decode_gqa_kv8(q[i: i + 1, :, :n].contiguous(), self.k_pools[layer], self.v_pools[layer], self.scales[layer],
+                                                         self.block_table[row: row + 1], lens, self.max_blocks_per_seq, softcap=softcap,
+                                                         mass=self.masses[layer], mass_index=index)
 
     def evict(self, request_ids: Sequence[str], budget: int, sink: int = 4, recent: int = 64) -> int:
         """Cut every request of more than `budget` committed tokens to `budget`, layer by layer and head by head; returns the blocks
@@ -398,6 +433,8 @@ class PagedKVCache8(BlockManager):
         ids = [r for r in request_ids if self._tokens[r] > budget]
         if not ids:
             return 0
+        for r in ids:                                             # tokens that were not committed are not kept
+            self._settle(r, 0)
         free = len(self._free)
         n = (budget + BLOCK_SIZE - 1) // BLOCK_SIZE
         blocks = self._take_blocks(n * len(ids))

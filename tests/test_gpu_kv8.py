@@ -841,6 +841,60 @@ def test_cache_class_serves_and_evicts(fa):
     assert c.get_num_free_blocks() == 64
 
 
+@pytest.mark.parametrize("codes", CODES)
+def test_cache_class_takes_rejected_guesses_back(fa, codes):
+    """The sums after steps of guesses are those of the tokens that stay; bfloat16, rotated."""
+    H, G, D = 2, 4, 64
+    lens = {"a": 100, "b": 37}
+    turn = lambda at: (torch.cos(at[:, None] * 0.01 * torch.arange(1, D // 2 + 1)), torch.sin(at[:, None] * 0.01 * torch.arange(1, D // 2 + 1)))
+
+    def step(c, names, counts, rows, kept, small=None):
+        for r in names:
+            c.reserve(r, c.get_cache_len(r) + counts)
+        at = torch.cat([torch.arange(counts) + c.position(r) for r in names]).float()
+        cos, sin = (torch.cat((t, t), 1).cuda() for t in turn(at))
+        cu = (torch.arange(len(names) + 1) * counts).int().cuda()
+        for layer, (q, k, v) in enumerate(rows):
+            q, k = c.append_prefill(layer, names, q.flatten(0, 1).contiguous(), k.flatten(0, 1).contiguous(), v.flatten(0, 1).contiguous(), cos, sin, cu)
+            out = c.attend(layer, names, q.view(len(names), counts, H * G, D).transpose(1, 2).contiguous(), softcap=20.0)
+            assert out.dtype == torch.bfloat16 and bool(out[:, :, 0].isfinite().all())
+        for r in names:
+            c.commit(r, kept[r])
+
+    def run(guesses):
+        c = fa.PagedKVCache8(40, 2, H, D, max_batch=3, max_blocks_per_seq=12, codes=codes)
+        c.allocate("x", 16)                                       # (so that the batches' rows of the table are gathered)
+        g = torch.Generator().manual_seed(150)
+        rnd = lambda *s: torch.randn(*s, generator=g).bfloat16().cuda()
+        for r, n in lens.items():
+            c.allocate(r, n)
+            step(c, [r], n, [[rnd(1, n, m, D) for m in (H * G, H, H)] for _ in range(2)], {r: n})
+        for kept in ({"a": 1, "b": 3}, {"a": 4, "b": 0}, {"a": 2, "b": 1}):
+            rows = [[rnd(2, 4, m, D) for m in (H * G, H, H)] for _ in range(2)]
+            for layer in rows:
+                for i, r in enumerate(("a", "b")):                # rejected rows ask for no larger scale
+                    layer[1][i, kept[r]:] *= 1e-3
+                    layer[2][i, kept[r]:] *= 1e-3
+            if guesses:
+                step(c, ["a", "b"], 4, rows, kept)
+            else:
+                for i, r in enumerate(("a", "b")):
+                    if kept[r]:
+                        step(c, [r], kept[r], [[t[i: i + 1, : kept[r]] for t in layer] for layer in rows], kept)
+        return c
+
+    got, want = run(True), run(False)
+    for layer in range(2):
+        # weights of one cache in calls of different batches: each off by 2^-17 at most (scores within 2^-18), the sums of a few of them by no more
+        assert bool(((got.masses[layer] - want.masses[layer]).abs() <= want.masses[layer] * 2.0 ** -16).all())
+        for r in lens:
+            assert bool((got.masses[layer][got.row_of(r), :, got.get_cache_len(r):] == 0).all())
+            own = torch.tensor(got.get_block_table(r))[: (got.get_cache_len(r) + 15) // 16]
+            other = torch.tensor(want.get_block_table(r))[: own.numel()]
+            assert torch.equal(got.scales[layer][own.cuda()], want.scales[layer][other.cuda()])
+    assert got._guessed == {} and got.get_cache_len("a") == 107 and got.get_cache_len("b") == 41
+
+
 # ---- the host side -------------------------------------------------------------------------------------------------
 def test_native_host_side_and_python_do_the_same(fa, monkeypatch):
     from flash_attn_v100_b200 import kv8_ops

@@ -140,3 +140,113 @@ def test_cache_class_bookkeeping():
         PagedKVCache8(8, 1, 2, 64, 2, 4, device="cpu", eviction=False).evict([], 10)
     with pytest.raises(ValueError):
         PagedKVCache8(8, 1, 2, 64, 2, 4, device="cpu", codes=torch.uint8)
+
+
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """The cache class with the oracle in the operators' place and no rotation."""
+    from flash_attn_v100_b200 import kv8_ops, ops
+
+    def append(k, v, k_cache, v_cache, scale, table, positions, width, cu_seqlens=None):
+        flat = lambda t: t.reshape(-1, t.size(1), t.size(-1)) if cu_seqlens is None else t
+        orc.append(flat(k), flat(v), k_cache, v_cache, scale, table, positions, cu_seqlens)
+
+    def decode(q, k_cache, v_cache, scale, table, lens, width, softcap=0.0, mass=None, mass_index=None):
+        sums = None if mass is None else mass.double()
+        out, _ = orc.decode(q, k_cache, v_cache, scale, table, lens.tolist(), softcap, sums, mass_index)
+        if mass is not None:
+            mass.copy_(sums)
+        return out.to(q.dtype)
+
+    def evict(mass, k_cache, v_cache, scale, table, lens, width, new, budget, sink=0, recent=0, mass_index=None):
+        return orc.evict(mass, k_cache, v_cache, scale, table, lens.tolist(), new, budget, sink, recent, mass_index)
+
+    monkeypatch.setattr(kv8_ops, "append_paged_kv8", append)
+    monkeypatch.setattr(kv8_ops, "forward_paged_decode_gqa_kv8", decode)
+    monkeypatch.setattr(kv8_ops, "evict_paged_kv8", evict)
+    monkeypatch.setattr(ops, "rope_append_paged_fp16", lambda q, k, *a, **kw: (q, k))
+    return decode
+
+
+def _serve(c, names, tokens, kept, g, small=1.0, spoiled=None):
+    """One step of `tokens` new tokens of each request, of which kept[name] stay; rows that do not are `small` times as large as others, and the query of
+    token `spoiled` is NaN."""
+    H, G, D = c.num_kv_heads, 2, c.head_dim
+    for r in names:
+        c.reserve(r, c.get_cache_len(r) + tokens)
+    factor = torch.ones(len(names), tokens)
+    for i, r in enumerate(names):
+        factor[i, kept[r]:] = small
+    for layer in range(c.num_layers):
+        q, k, v = (torch.randn(len(names) * tokens, n, D, generator=g).half() for n in (H * G, H, H))
+        k, v = ((t * factor.reshape(-1, 1, 1)).half() for t in (k, v))
+        cu = torch.arange(0, len(names) * tokens + 1, tokens, dtype=torch.int32)
+        q, k = c.append_prefill(layer, names, *(t.to(c.device) for t in (q, k, v)), None, None, cu.to(c.device))
+        q = q.view(len(names), tokens, H * G, D).transpose(1, 2).contiguous()
+        if spoiled is not None:
+            q[:, :, spoiled] = math.nan
+        c.attend(layer, names, q)
+    for r in names:
+        c.commit(r, kept[r])
+
+
+def test_weights_of_rejected_guesses_are_taken_back(on_cpu):
+    """Steps of four guesses, of which some stay, leave the sums that the tokens that stay have given alone; also slots that are written again, and a NaN."""
+    from flash_attn_v100_b200 import PagedKVCache8
+    lens = {"a": 20, "b": 33}
+
+    def run(guesses):
+        c = PagedKVCache8(20, 2, 2, 64, max_batch=3, max_blocks_per_seq=6, device="cpu")
+        g = torch.Generator().manual_seed(7)
+        for r, n in lens.items():
+            c.allocate(r, n)
+            _serve(c, [r], n, {r: n}, g)
+        c.allocate("c", 16)                                       # (a row that nobody touches)
+        c.masses[1][c.row_of("c")] = 3.0
+        for step, kept in enumerate(({"a": 1, "b": 3}, {"a": 4, "b": 0}, {"a": 0, "b": 1}, {"a": 2, "b": 4})):
+            g = torch.Generator().manual_seed(step)
+            if guesses:
+                _serve(c, ["a", "b"], 4, kept, g, small=1e-3, spoiled=3 if step == 0 else None)
+            else:
+                # the same tokens, but those that do not stay are never there: a request at a time
+                H, G, D = 2, 2, 64
+                drawn = [[torch.randn(8, n, D, generator=g).half().view(2, 4, n, D) for n in (H * G, H, H)] for _ in range(2)]
+                for i, r in enumerate(("a", "b")):
+                    n = kept[r]
+                    if n == 0:
+                        continue
+                    c.reserve(r, c.get_cache_len(r) + n)
+                    for layer in range(2):
+                        q, k, v = (t[i, :n] for t in drawn[layer])
+                        c.append_prefill(layer, [r], q, k, v, None, None, torch.tensor([0, n], dtype=torch.int32))
+                        c.attend(layer, [r], q.transpose(0, 1)[None].contiguous())
+                    c.commit(r, n)
+        return c
+
+    got, want = run(True), run(False)
+    assert got._guessed == {} and got.get_cache_len("a") == want.get_cache_len("a") == 27
+    for layer in range(2):
+        assert bool(got.masses[layer].isfinite().all())
+        # the class's sums are fp32: of about ten additions each is off by at most 2^-24 of a sum; the codes are the same, as rejected rows are small
+        assert bool(((got.masses[layer] - want.masses[layer]).abs() <= want.masses[layer] * 2.0 ** -20).all())
+        for r, n in (("a", 27), ("b", 41)):
+            assert bool((got.masses[layer][got.row_of(r), :, n:] == 0).all())
+    got.release("a")
+    assert "a" not in got._guessed
+
+
+def test_an_eviction_drops_what_was_not_committed(on_cpu):
+    from flash_attn_v100_b200 import PagedKVCache8
+    c = PagedKVCache8(20, 1, 2, 64, max_batch=1, max_blocks_per_seq=6, device="cpu")
+    g = torch.Generator().manual_seed(8)
+    c.allocate("a", 40)
+    _serve(c, ["a"], 40, {"a": 40}, g)
+    sums = c.masses[0].clone()
+    c.reserve("a", 43)
+    q, k, v = (torch.randn(3, n, 64, generator=g).half() for n in (4, 2, 2))
+    c.append_prefill(0, ["a"], q, k, v, None, None, torch.tensor([0, 3], dtype=torch.int32))
+    c.attend(0, ["a"], q.transpose(0, 1)[None].contiguous())
+    assert not torch.equal(c.masses[0], sums)
+    c.evict(["a"], 20, 2, 4)
+    kept = torch.tensor([orc.choose(sums[0, h].tolist(), 40, 20, 2, 4) for h in range(2)])
+    assert torch.equal(c.masses[0][0, :, :20], sums[0].gather(1, kept)) and bool((c.masses[0][0, :, 20:] == 0).all()) and c._guessed == {}
