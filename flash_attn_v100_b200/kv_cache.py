@@ -28,7 +28,7 @@ need no prefill (the reference's `allocate` documents this and does not do it, m
 from __future__ import annotations
 
 import hashlib
-from typing import Dict, List, Optional, Sequence, Set
+from typing import Dict, List, NamedTuple, Optional, Sequence, Set
 
 import torch
 
@@ -302,6 +302,30 @@ class PagedKVCache(BlockManager):
                                           self.max_blocks_per_seq, cu_seqlens=cu_seqlens, return_k=True)
 
 
+class _Offsets:
+    """Offsets of a batch's packed rows as they were at its append; on the host once they are asked for."""
+
+    def __init__(self, cu_seqlens):
+        self.source, self.version = cu_seqlens, cu_seqlens._version
+        self._copy, self._list = cu_seqlens.clone(), None
+
+    def is_of(self, cu_seqlens) -> bool:
+        return self.source is cu_seqlens and self.version == cu_seqlens._version
+
+    def rows(self, i: int):
+        if self._list is None:
+            self._list = self._copy.tolist()
+        return self._list[i], self._list[i + 1]
+
+
+class _Appended(NamedTuple):
+    """Rows of an append whose tokens may not all stay, and the blocks that they went on in as these were before."""
+    offsets: _Offsets
+    k: torch.Tensor
+    v: torch.Tensor
+    blocks: Sequence[torch.Tensor]                               # codes of k and v [B, H_KV, 16, D] and scales [B, H_KV, 2]
+
+
 class PagedKVCache8(BlockManager):
     """K and V pools in 8 bits, `[num_blocks, H_KV, 16, D]` per layer with a scale for each block, head and kind, and eviction by
     the weights that attention gave the tokens.
@@ -310,8 +334,8 @@ class PagedKVCache8(BlockManager):
     tokens, [max_batch, H_KV, tokens] in fp32, which `attend` adds to and `evict` goes by.  A request that was cut has
     `get_cache_len` tokens in the cache and `position` tokens behind it: rotary angles go by the latter.
 
-    Guessed tokens are appended and attended to together; `commit` takes how many of them stay, and the weights that the others gave are
-    taken back.  (Their rows are written over by the next tokens.  The scale that they asked of a block they share with tokens that stay is not taken back.)"""
+    Guessed tokens are appended (`append_prefill`, up to 16 for a request on average) and attended to together; `commit` takes how many of them stay, and the
+    cache and the sums become what those alone make them: a block that was begun before gets its codes and scales back."""
 
     def __init__(self, num_blocks: int, num_layers: int, num_kv_heads: int, head_dim: int, max_batch: int, max_blocks_per_seq: int,
                  device="cuda", codes=torch.int8, enable_prefix_cache: bool = True, eviction: bool = True):
@@ -329,8 +353,11 @@ class PagedKVCache8(BlockManager):
         self.masses = [torch.zeros((max_batch, num_kv_heads, max_blocks_per_seq * BLOCK_SIZE), device=self.device)
                        for _ in range(num_layers)] if eviction else None
         self._positions: Dict[str, int] = {}                     # request -> tokens it has had
-        # request -> layer -> attentions of several tokens that are not committed: (place in the batch, the batch's sums before the first, q, softcap)
+        # What a commit of fewer tokens than there were goes by, request -> layer: the last append (place in the batch, batch), what was before the first
+        # (likewise), and attentions (place in the batch, the batch's sums before the first, q, softcap)
+        self._appended: Dict[str, Dict[int, tuple]] = {}
         self._guessed: Dict[str, Dict[int, list]] = {}
+        self._offsets: Optional[_Offsets] = None
 
     # ---- bookkeeping ----------------------------------------------------------------
     def allocate(self, request_id: str, num_tokens: int = 0, token_ids: Optional[Sequence[int]] = None) -> int:
@@ -341,8 +368,8 @@ class PagedKVCache8(BlockManager):
         return row
 
     def commit(self, request_id: str, num_new_tokens: int) -> None:
-        """Advance the token count by the appended tokens that stay.  Where `attend` has added the weights of more than those to the sums, they are
-        put back and those of the tokens that stay are added again."""
+        """Advance the token count by the appended tokens that stay.  Where there were more, blocks and sums are put back to what they were before, and
+        the rows and weights of the tokens that stay are added again."""
         super().commit(request_id, num_new_tokens)
         self._positions[request_id] += num_new_tokens
         self._settle(request_id, num_new_tokens)
@@ -350,6 +377,7 @@ class PagedKVCache8(BlockManager):
     def release(self, request_id: str) -> None:
         super().release(request_id)
         self._positions.pop(request_id, None)
+        self._appended.pop(request_id, None)
         self._guessed.pop(request_id, None)
 
     def position(self, request_id: str) -> int:
@@ -367,8 +395,20 @@ class PagedKVCache8(BlockManager):
         table, lens = self.batch_view(request_ids)
         rotate = ops.rope_append_paged_bf16 if q.dtype == torch.bfloat16 else ops.rope_append_paged_fp16
         q, k = rotate(q, k, v, cos, sin, None, None, None, lens if cu_seqlens is None else None, 0, cu_seqlens=cu_seqlens, return_k=True)
+        # Guesses are a few tokens of each request; the rows of longer prompts are not kept, as all of them stay.
+        guess = cu_seqlens is not None and 0 < k.size(0) <= BLOCK_SIZE * len(request_ids)
+        if guess:
+            if self._offsets is None or not self._offsets.is_of(cu_seqlens):
+                self._offsets = _Offsets(cu_seqlens)
+            begun = table.gather(1, (lens // BLOCK_SIZE).clamp(max=self.max_blocks_per_seq - 1).long()[:, None])[:, 0].clamp(min=0)
+            blocks = [t.view(torch.int8)[begun] for t in (self.k_pools[layer], self.v_pools[layer])] + [self.scales[layer][begun]]
+            batch = _Appended(self._offsets, k, v.clone(memory_format=torch.contiguous_format), blocks)
         kv8_ops.append_paged_kv8(k, v, self.k_pools[layer], self.v_pools[layer], self.scales[layer], table, lens, self.max_blocks_per_seq,
                                  cu_seqlens=cu_seqlens)
+        if guess:
+            for i, r in enumerate(request_ids):
+                layers = self._appended.setdefault(r, {})
+                layers[layer] = ((i, batch), layers[layer][1] if layer in layers else (i, batch))
         return q, k
 
     def append_decode(self, layer: int, request_ids: Sequence[str], q, k, v, cos, sin):
@@ -402,22 +442,34 @@ class PagedKVCache8(BlockManager):
         return out
 
     def _settle(self, request_id: str, kept: int) -> None:
-        """The sums of weights as if only the first `kept` (committed by now) of the tokens attended to since the last commit had been there."""
+        """Blocks and sums of weights as if only the first `kept` (committed by now) of the tokens since the last commit had been there."""
         from . import kv8_ops
+        appended, guessed = self._appended.pop(request_id, {}), self._guessed.pop(request_id, {})
         row, held = self._row[request_id], self._tokens[request_id] - kept
-        for layer, calls in self._guessed.pop(request_id, {}).items():
+        table, ints = self.block_table[row: row + 1], lambda v: torch.tensor(v, dtype=torch.int32).to(self.device)
+        for layer in sorted({*appended, *guessed}):
+            pools = (self.k_pools[layer], self.v_pools[layer], self.scales[layer])
+            if layer in appended:
+                (i, last), (j, first) = appended[layer]
+                begin, end = last.offsets.rows(i)
+                if kept < end - begin:
+                    if held % BLOCK_SIZE:
+                        block = self._tables[request_id][held // BLOCK_SIZE]
+                        for pool, before in zip(pools, first.blocks):
+                            pool[block] = before[j].view(pool.dtype)
+                    if kept > 0:
+                        kv8_ops.append_paged_kv8(last.k[begin: begin + kept], last.v[begin: begin + kept], *pools, table, ints([held]), self.max_blocks_per_seq,
+                                                 cu_seqlens=ints([0, kept]))
+            calls = guessed.get(layer, ())
             if all(q.size(2) <= kept for _, _, q, _ in calls):
                 continue
             i, before, _, _ = calls[0]
             self.masses[layer][row, :, : before.size(2)] = before[i]
-            index = torch.tensor([row], dtype=torch.int32).to(self.device)
             for i, _, q, softcap in calls:
                 n = min(kept, q.size(2))
                 if n > 0:
-                    lens = torch.tensor([held + n], dtype=torch.int32).to(self.device)
-                    kv8_ops.forward_paged_decode_gqa_kv8(q[i: i + 1, :, :n].contiguous(), self.k_pools[layer], self.v_pools[layer], self.scales[layer],
-                                                         self.block_table[row: row + 1], lens, self.max_blocks_per_seq, softcap=softcap,
-                                                         mass=self.masses[layer], mass_index=index)
+                    kv8_ops.forward_paged_decode_gqa_kv8(q[i: i + 1, :, :n].contiguous(), *pools, table, ints([held + n]), self.max_blocks_per_seq, softcap=softcap,
+                                                         mass=self.masses[layer], mass_index=ints([row]))
 
     def evict(self, request_ids: Sequence[str], budget: int, sink: int = 4, recent: int = 64) -> int:
         """Cut every request of more than `budget` committed tokens to `budget`, layer by layer and head by head; returns the blocks

@@ -895,6 +895,52 @@ def test_cache_class_takes_rejected_guesses_back(fa, codes):
     assert got._guessed == {} and got.get_cache_len("a") == 107 and got.get_cache_len("b") == 41
 
 
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("bad", [40.0, math.nan])
+def test_cache_class_gives_begun_blocks_back(fa, codes, bad):
+    """Rejected rows that ask for a larger scale, or spoil a block: codes and scales are bit for bit those of a run without them."""
+    H, D = 2, 128
+
+    def run(guesses):
+        c = fa.PagedKVCache8(40, 2, H, D, max_batch=3, max_blocks_per_seq=12, codes=codes)
+        g = torch.Generator().manual_seed(151)
+        rnd = lambda *s: torch.randn(*s, generator=g).half().cuda()
+        turn = lambda n: (torch.ones(n, D).cuda(), torch.zeros(n, D).cuda())      # no rotation
+        put = lambda layer, names, rows, cu: c.append_prefill(layer, names, *rows, *turn(rows[0].size(0)), _ints(cu).cuda())
+        for r, n in (("a", 100), ("b", 37)):
+            c.allocate(r, n)
+            for layer in range(2):
+                put(layer, [r], [rnd(n, m, D) for m in (2 * H, H, H)], [0, n])
+            c.commit(r, n)
+        for kept in ({"a": 1, "b": 2}, {"a": 0, "b": 3}, {"a": 5, "b": 0}):
+            for r in "ab":
+                c.reserve(r, c.get_cache_len(r) + 5)
+            for layer in range(2):
+                rows = [rnd(8, m, D) for m in (2 * H, H, H)]
+                if guesses:
+                    for t in rows[1:]:
+                        t[kept["a"]: 5], t[5 + kept["b"]:] = bad, bad
+                    put(layer, ["a", "b"], rows, [0, 5, 8])
+                else:
+                    for r, at in (("a", 0), ("b", 5)):
+                        if kept[r]:
+                            put(layer, [r], [t[at: at + kept[r]] for t in rows], [0, kept[r]])
+            for r in "ab":
+                c.commit(r, kept[r])
+        return c
+
+    got, want = run(True), run(False)
+    for r in "ab":
+        n = got.get_cache_len(r)
+        assert n == want.get_cache_len(r)
+        own, other = (torch.tensor(c.get_block_table(r)[: (n + 15) // 16]).cuda() for c in (got, want))
+        for layer in range(2):
+            assert torch.equal(got.scales[layer][own], want.scales[layer][other])
+            for a, b in ((got.k_pools, want.k_pools), (got.v_pools, want.v_pools)):
+                a, b = (kc.bits(t[layer])[at].transpose(1, 2).flatten(0, 1)[:n] for t, at in ((a, own), (b, other)))
+                assert torch.equal(a, b)
+
+
 # ---- the host side -------------------------------------------------------------------------------------------------
 def test_native_host_side_and_python_do_the_same(fa, monkeypatch):
     from flash_attn_v100_b200 import kv8_ops

@@ -250,3 +250,60 @@ def test_an_eviction_drops_what_was_not_committed(on_cpu):
     c.evict(["a"], 20, 2, 4)
     kept = torch.tensor([orc.choose(sums[0, h].tolist(), 40, 20, 2, 4) for h in range(2)])
     assert torch.equal(c.masses[0][0, :, :20], sums[0].gather(1, kept)) and bool((c.masses[0][0, :, 20:] == 0).all()) and c._guessed == {}
+
+
+@pytest.mark.parametrize("bad", [30.0, math.inf, math.nan])
+def test_rejected_guesses_leave_no_trace_in_their_blocks(on_cpu, bad):
+    """Rows that do not stay and ask for a larger scale, or spoil a block, leave codes, scales and sums as they are without them; also where a request is evicted instead."""
+    from flash_attn_v100_b200 import PagedKVCache8
+    H, D = 2, 64
+
+    def run(guesses):
+        c = PagedKVCache8(20, 2, H, D, max_batch=2, max_blocks_per_seq=6, device="cpu", codes=torch.float8_e4m3fn)
+        for r, n in (("a", 20), ("b", 37)):
+            c.allocate(r, n)
+            _serve(c, [r], n, {r: n}, torch.Generator().manual_seed(n))
+        cu = torch.tensor([0, 5, 8], dtype=torch.int32)
+        for step, kept in enumerate(({"a": 1, "b": 2}, {"a": 0, "b": 3}, {"a": 5, "b": 0})):
+            g = torch.Generator().manual_seed(step)
+            rows = [[torch.randn(8, n, D, generator=g).half() for n in (2 * H, H, H)] for _ in range(2)]
+            for r in ("a", "b"):
+                c.reserve(r, c.get_cache_len(r) + 5)
+            for layer in range(2):
+                if guesses:
+                    q, k, v = (t.clone() for t in rows[layer])
+                    for t in (k, v):
+                        t[kept["a"]: 5], t[5 + kept["b"]:] = bad, bad
+                    c.append_prefill(layer, ["a", "b"], q, k, v, None, None, cu)
+                    v.zero_()                                     # (the caller's rows may change behind the call)
+                else:
+                    for r, at in (("a", 0), ("b", 5)):
+                        q, k, v = (t[at: at + kept[r]] for t in rows[layer])
+                        if kept[r]:
+                            c.append_prefill(layer, [r], q, k, v, None, None, torch.tensor([0, kept[r]], dtype=torch.int32))
+            cu.zero_()                                            # (so may its offsets)
+            for r in ("a", "b"):
+                c.commit(r, kept[r])
+            cu.copy_(torch.tensor([0, 5, 8]))
+        return c
+
+    got, want = run(True), run(False)
+    assert got._appended == {} and [got.get_cache_len(r) for r in "ab"] == [want.get_cache_len(r) for r in "ab"] == [26, 42]
+    for layer in range(2):
+        for r in "ab":
+            n = got.get_cache_len(r)
+            blocks = [c.get_block_table(r)[: (n + 15) // 16] for c in (got, want)]
+            for i, name in enumerate(("k_pools", "v_pools")):
+                for h in range(H):
+                    a, b = (orc.rows_of(getattr(c, name)[layer], c.scales[layer], i, t, h, n) for c, t in zip((got, want), blocks))
+                    assert torch.equal(a, b)
+            assert torch.equal(got.scales[layer][blocks[0]], want.scales[layer][blocks[1]])
+    # tokens that were appended to begun blocks and not committed are gone with an eviction
+    c = got
+    c.reserve("a", 28)
+    rows = [torch.full((2, n, D), bad).half() for n in (2 * H, H, H)]
+    for layer in range(2):
+        c.append_prefill(layer, ["a"], *rows, None, None, torch.tensor([0, 2], dtype=torch.int32))
+    c.evict(["a"], 25, 1, 20)
+    t = c.get_block_table("a")
+    assert bool(c.scales[0][t].isfinite().all()) and float(c.scales[0][t].max()) < 0.03      # (30 / 448 is more)
