@@ -485,26 +485,29 @@ class PagedKVCache8(BlockManager):
         ids = [r for r in request_ids if self._tokens[r] > budget]
         if not ids:
             return 0
-        for r in ids:                                             # tokens that were not committed are not kept
-            self._settle(r, 0)
         free = len(self._free)
         n = (budget + BLOCK_SIZE - 1) // BLOCK_SIZE
         blocks = self._take_blocks(n * len(ids))
         new = [blocks[i * n: (i + 1) * n] for i in range(len(ids))]
         try:
+            for r in ids:                                         # tokens that were not committed are not kept
+                self._settle(r, 0)
             table, lens = self.batch_view(ids)
             new_table = torch.tensor(new, dtype=torch.int32).to(self.device)
             rows = torch.tensor([self._row[r] for r in ids], dtype=torch.int32).to(self.device)
-            at = rows.long()
+            sums = []
             for layer in range(self.num_layers):
-                mass = self.masses[layer]
-                _, _, kept = kv8_ops.evict_paged_kv8(mass, self.k_pools[layer], self.v_pools[layer], self.scales[layer], table, lens,
+                _, _, kept = kv8_ops.evict_paged_kv8(self.masses[layer], self.k_pools[layer], self.v_pools[layer], self.scales[layer], table, lens,
                                                      self.max_blocks_per_seq, new_table, budget, sink, recent, mass_index=rows)
-                mass[at] = torch.nn.functional.pad(kept, (0, mass.size(2) - budget))
+                sums.append(kept)
+            at = rows.long()
+            sums = [torch.nn.functional.pad(kept, (0, mass.size(2) - budget)) for kept, mass in zip(sums, self.masses)]
         except Exception:
             for b in reversed(blocks):
                 self._drop_ref(b)
             raise
+        for mass, kept in zip(self.masses, sums):                 # (once no layer can fail any more: until here everything is as it was)
+            mass[at] = kept
         for r, own in zip(ids, new):
             row, old = self._row[r], self._tables[r]
             self._tables[r] = list(own)

@@ -307,3 +307,31 @@ def test_rejected_guesses_leave_no_trace_in_their_blocks(on_cpu, bad):
     c.evict(["a"], 25, 1, 20)
     t = c.get_block_table("a")
     assert bool(c.scales[0][t].isfinite().all()) and float(c.scales[0][t].max()) < 0.03      # (30 / 448 is more)
+
+
+def test_an_eviction_that_fails_leaves_the_sums(on_cpu, monkeypatch):
+    """A layer that fails behind others: sums, tokens and blocks of all layers are as they were, and a second try cuts as if there had been no first."""
+    from flash_attn_v100_b200 import PagedKVCache8, kv8_ops
+    c = PagedKVCache8(20, 3, 2, 64, max_batch=2, max_blocks_per_seq=6, device="cpu")
+    for r, n in (("a", 40), ("b", 57)):
+        c.allocate(r, n)
+        _serve(c, [r], n, {r: n}, torch.Generator().manual_seed(n))
+    before, free, tables = [m.clone() for m in c.masses], c.get_num_free_blocks(), [c.get_block_table(r) for r in "ab"]
+    evict, calls = kv8_ops.evict_paged_kv8, []
+
+    def failing(*a, **kw):
+        calls.append(a)
+        if len(calls) == 2:
+            raise torch.OutOfMemoryError("no room for the second layer")
+        return evict(*a, **kw)
+
+    monkeypatch.setattr(kv8_ops, "evict_paged_kv8", failing)
+    with pytest.raises(torch.OutOfMemoryError):
+        c.evict(["a", "b"], 20, 2, 4)
+    assert all(torch.equal(m, b) for m, b in zip(c.masses, before)) and c.get_num_free_blocks() == free
+    assert [c.get_block_table(r) for r in "ab"] == tables and (c.get_cache_len("a"), c.get_cache_len("b")) == (40, 57)
+    c.evict(["a", "b"], 20, 2, 4)
+    for layer in range(3):
+        for row, n in ((c.row_of("a"), 40), (c.row_of("b"), 57)):
+            kept = torch.tensor([orc.choose(before[layer][row, h].tolist(), n, 20, 2, 4) for h in range(2)])
+            assert torch.equal(c.masses[layer][row, :, :20], before[layer][row].gather(1, kept)) and bool((c.masses[layer][row, :, 20:] == 0).all())
