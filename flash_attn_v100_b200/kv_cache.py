@@ -500,14 +500,14 @@ class PagedKVCache8(BlockManager):
                 _, _, kept = kv8_ops.evict_paged_kv8(self.masses[layer], self.k_pools[layer], self.v_pools[layer], self.scales[layer], table, lens,
                                                      self.max_blocks_per_seq, new_table, budget, sink, recent, mass_index=rows)
                 sums.append(kept)
-            at = rows.long()
-            sums = [torch.nn.functional.pad(kept, (0, mass.size(2) - budget)) for kept, mass in zip(sums, self.masses)]
+            at, held = rows.long(), max(len(self._tables[r]) for r in ids) * BLOCK_SIZE
         except Exception:
             for b in reversed(blocks):
                 self._drop_ref(b)
             raise
         for mass, kept in zip(self.masses, sums):                 # (once no layer can fail any more: until here everything is as it was)
-            mass[at] = kept
+            mass[at, :, :budget] = kept
+            mass[at, :, budget:held] = 0.0
         for r, own in zip(ids, new):
             row, old = self._row[r], self._tables[r]
             self._tables[r] = list(own)
