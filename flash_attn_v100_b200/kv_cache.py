@@ -473,19 +473,37 @@ class PagedKVCache8(BlockManager):
 
     def evict(self, request_ids: Sequence[str], budget: int, sink: int = 4, recent: int = 64) -> int:
         """Cut every request of more than `budget` committed tokens to `budget`, layer by layer and head by head; returns the blocks
-        that came free (less than 0 where shared ones stay held).  The tokens move to new blocks, so blocks that other requests or a prefix share stay as they are; there must
-        be enough free ones for the requests that are cut."""
-        from . import kv8_ops
+        that came free (less than 0 where shared ones stay held).  The tokens move to new blocks, so blocks that other requests or a prefix share stay as they are.
+        Requests are cut in turns where there are not enough free blocks for all at once; where one could not be cut, MemoryError is raised before any is.
+        Tokens that are not committed are not kept."""
         if self.masses is None:
             raise RuntimeError("this cache keeps no sums of weights (eviction=False)")
         if budget <= 0 or sink < 0 or recent < 0 or sink + recent > budget:
             raise ValueError("budget must be positive and hold sink and recent")
         if len(set(request_ids)) != len(request_ids):
             raise ValueError("a request is named twice")
-        ids = [r for r in request_ids if self._tokens[r] > budget]
-        if not ids:
-            return 0
         free = len(self._free)
+        for ids in self._turns([r for r in request_ids if self._tokens[r] > budget], (budget + BLOCK_SIZE - 1) // BLOCK_SIZE):
+            self._cut(ids, budget, sink, recent)
+        return len(self._free) - free
+
+    def _turns(self, ids: Sequence[str], n: int) -> List[List[str]]:
+        """The requests in as few runs, in order, as free blocks allow if each takes n and the blocks that nobody else holds come free behind its run."""
+        turns, free, refs, at = [], len(self._free), {}, 0
+        while at < len(ids):
+            turn = list(ids[at: at + free // n])
+            if not turn:
+                raise MemoryError(f"paged KV cache exhausted: need {n} blocks to cut request {ids[at]!r}, {free} free")
+            free -= n * len(turn)
+            for b in (b for r in turn for b in self._tables[r] if b >= 0):
+                refs[b] = refs.get(b, self._refs[b]) - 1
+                free += refs[b] == 0
+            turns.append(turn)
+            at += len(turn)
+        return turns
+
+    def _cut(self, ids: Sequence[str], budget: int, sink: int, recent: int) -> None:
+        from . import kv8_ops
         n = (budget + BLOCK_SIZE - 1) // BLOCK_SIZE
         blocks = self._take_blocks(n * len(ids))
         new = [blocks[i * n: (i + 1) * n] for i in range(len(ids))]
@@ -517,7 +535,6 @@ class PagedKVCache8(BlockManager):
             for b in reversed(old):
                 if b >= 0:
                     self._drop_ref(b)
-        return len(self._free) - free
 
 
 class HybridCache(BlockManager):

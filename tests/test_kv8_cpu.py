@@ -335,3 +335,42 @@ def test_an_eviction_that_fails_leaves_the_sums(on_cpu, monkeypatch):
         for row, n in ((c.row_of("a"), 40), (c.row_of("b"), 57)):
             kept = torch.tensor([orc.choose(before[layer][row, h].tolist(), n, 20, 2, 4) for h in range(2)])
             assert torch.equal(c.masses[layer][row, :, :20], before[layer][row].gather(1, kept)) and bool((c.masses[layer][row, :, 20:] == 0).all())
+
+
+def test_an_eviction_of_a_nearly_full_cache_goes_in_turns(on_cpu):
+    """Blocks that the first requests give back are those that the next ones move to; where even that does not do, nothing is touched."""
+    from flash_attn_v100_b200 import PagedKVCache8
+    lens = {"a": 90, "b": 96, "c": 81, "d": 30}
+
+    def filled(blocks):
+        c = PagedKVCache8(blocks, 2, 2, 64, max_batch=4, max_blocks_per_seq=6, device="cpu")
+        for r, n in lens.items():
+            c.allocate(r, n)
+            _serve(c, [r], n, {r: n}, torch.Generator().manual_seed(n))
+        return c
+
+    got, want = filled(22), filled(60)                            # 20 blocks are held, a cut request takes two
+    assert got.evict(list("abcd"), 32, 2, 8) == want.evict(list("abcd"), 32, 2, 8) == 12
+    assert got.get_num_free_blocks() == 14 and sum(got._refs) == 8 and sorted(got._free + [b for r in lens for b in got.get_block_table(r)]) == list(range(22))
+    for r, n in lens.items():
+        n = min(n, 32)
+        assert got.get_cache_len(r) == n and got.position(r) == lens[r]
+        tables = [c.get_block_table(r) for c in (got, want)]
+        assert got.block_table[got.row_of(r)].tolist() == tables[0] + [-1] * (6 - len(tables[0]))
+        for layer in range(2):
+            assert torch.equal(got.masses[layer], want.masses[layer])
+            for i, name in enumerate(("k_pools", "v_pools")):
+                a, b = (orc.rows_of(getattr(c, name)[layer], c.scales[layer], i, t, 1, n) for c, t in zip((got, want), tables))
+                assert torch.equal(a, b)
+    # four blocks for a request and two free ones; and blocks that a prefix holds do not come free
+    c = filled(22)
+    state = lambda: (c._free[:], {r: c.get_block_table(r) for r in lens}, [m.clone() for m in c.masses])
+    before = state()
+    with pytest.raises(MemoryError):
+        c.evict(list("abcd"), 50, 2, 8)
+    assert c.cache_prefix(list(range(90)), "a") == 80
+    with pytest.raises(MemoryError):
+        c.evict(["a", "b"], 32, 2, 8)
+    after = state()
+    assert after[:2] == before[:2] and all(torch.equal(x, y) for x, y in zip(after[2], before[2]))
+    assert c.evict(["b", "a"], 32, 2, 8) == 4 - 1                  # five of a's six blocks stay held by the prefix
