@@ -18,6 +18,7 @@ from .ops import (PAGE_BLOCK_SIZE, SUPPORTED_D, _check_dim, _check_gqa_heads, _c
 
 _ROWS = {torch.float16: 0, torch.bfloat16: 1}
 _CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
+_INT = 2 ** 31 - 1      # the C ABI's sizes
 _call_mod = _UNSET
 
 
@@ -57,7 +58,7 @@ def _cache(k_cache, v_cache, kv_scale, block_table, batch, max_num_blocks):
     _chk(block_table.dtype == torch.int32 and block_table.dim() == 2, "block_table must be a 2D int32 tensor")
     _chk(block_table.size(0) >= batch, "block_table batch size must match")
     max_num_blocks = int(max_num_blocks)
-    _chk(max_num_blocks > 0, "max_num_blocks must be positive")
+    _chk(0 < max_num_blocks <= _INT, "max_num_blocks must be positive and below 2^31")
     used = min(max_num_blocks, block_table.size(1))
     _chk(used > 0 and (batch - 1) * max_num_blocks + used <= block_table.numel(), "max_num_blocks (row stride) is larger than block_table allows")
     return _lib.Kv8Cache(k=_ptr(k_cache), v=_ptr(v_cache), scale=_ptr(kv_scale), pages=pages, heads=heads, dim=dim, codes=_CODES[k_cache.dtype],
@@ -123,6 +124,7 @@ def _check_mass(mass, mass_index, batch, c, like):
     _check_input(mass, "mass")
     _same_device(like, mass, "k_cache", "mass")
     _chk(mass.dtype == torch.float32 and mass.dim() == 3 and mass.size(1) == c.heads, "mass must be float32 [rows, H_KV, tokens]")
+    _chk(max(mass.size(0), mass.size(2)) <= _INT, "mass must have fewer than 2^31 rows and tokens")
     _chk(mass.size(2) >= c.max_pages * PAGE_BLOCK_SIZE, "mass must have room for every token of a block_table row")
     if mass_index is None:
         _chk(mass.size(0) >= batch, "mass must have a row for each sequence")
@@ -190,6 +192,7 @@ def evict_paged_kv8(mass, k_cache, v_cache, kv_scale, block_table, seq_lens, max
     budget, sink, recent = int(budget), int(sink), int(recent)
     _chk(budget > 0 and sink >= 0 and recent >= 0 and sink + recent <= budget, "budget must be positive and hold sink and recent")
     _chk(new_block_table.dtype == torch.int32 and new_block_table.dim() == 2 and new_block_table.size(0) >= batch, "new_block_table must be int32 [B, *]")
+    _chk(max(budget, new_block_table.size(1)) <= _INT, "budget and the rows of new_block_table must be below 2^31")
     _chk(new_block_table.size(1) * PAGE_BLOCK_SIZE >= budget, "new_block_table must have room for budget tokens")
     with _on(k_cache.device):
         kept = torch.empty((batch, c.heads, budget), dtype=torch.int32, device=k_cache.device)

@@ -374,3 +374,24 @@ def test_an_eviction_of_a_nearly_full_cache_goes_in_turns(on_cpu):
     after = state()
     assert after[:2] == before[:2] and all(torch.equal(x, y) for x, y in zip(after[2], before[2]))
     assert c.evict(["b", "a"], 32, 2, 8) == 4 - 1                  # five of a's six blocks stay held by the prefix
+
+
+def test_sizes_beyond_32_bits_are_refused(monkeypatch):
+    """What the C ABI takes as 32-bit numbers would be cut off: refused before a call (shapes only, no memory)."""
+    from flash_attn_v100_b200 import _lib, kv8_ops
+    for name in ("_check_input", "_same_device"):
+        monkeypatch.setattr(kv8_ops, name, lambda *a: None)
+    monkeypatch.setattr(kv8_ops, "_native", lambda *a: None)
+    monkeypatch.setattr(_lib, "library", lambda name: pytest.fail("called"))
+    meta = lambda shape, dtype: torch.empty(shape, dtype=dtype, device="meta")
+    k8, scale, lens = meta((4, 2, 16, 64), torch.int8), meta((4, 2, 2), torch.float32), meta(1, torch.int32)
+    table, mass, new = meta((1, 2), torch.int32), meta((1, 2, 32), torch.float32), meta((1, 1), torch.int32)
+    big = 2 ** 32 + 64
+    evict = lambda mass=mass, width=2, new=new, budget=16: kv8_ops.evict_paged_kv8(mass, k8, k8, scale, table, lens, width, new, budget)
+    for call, message in ((lambda: evict(mass=meta((1, 2, big), torch.float32)), "fewer than 2.31 rows"),
+                          (lambda: evict(mass=meta((big, 2, 32), torch.float32)), "fewer than 2.31 rows"),
+                          (lambda: evict(new=meta((1, big), torch.int32)), "below 2.31"),
+                          (lambda: evict(new=meta((1, big), torch.int32), budget=big), "below 2.31"),
+                          (lambda: evict(width=big), "below 2.31")):
+        with pytest.raises(RuntimeError, match=message):
+            call()
