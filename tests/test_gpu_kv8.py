@@ -489,6 +489,13 @@ def test_decode_of_queries_with_one_large_element(fa, codes, D, power):
     assert bool((off <= bound).all()), (off / bound).max().item()
 
 
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("D,H,G,T", [(64, 1, 4, 64), (128, 2, 2, 100), (256, 1, 3, 70)])
+def test_decode_of_many_rows(fa, codes, D, H, G, T):
+    """Hundreds of rows of a KV head: many blocks, whose tokens see more and more of the last pages."""
+    _decode_case(fa, codes, torch.float16, H, G, D, T, [0, 1, T, T + 30, 300], 145, mass=True)
+
+
 def test_caches_of_more_than_32_bits(fa):
     """Pages whose codes lie beyond 2^32 bytes."""
     H, D, lens = 8, 256, [50]
@@ -653,6 +660,28 @@ def test_prompts_steps_and_eviction_in_a_row(fa, codes):
     mass64[:, :, :budget] = new_mass.cpu().double()
     lens = steps(20, new, new_lens.tolist())
     assert lens == [60, 58, 60]
+
+
+@pytest.mark.parametrize("codes", CODES)
+def test_sums_of_many_steps(fa, codes):
+    """Sums that twenty steps add to stay within what each step's scores and roundings allow."""
+    H, G, D, lens = 2, 4, 128, [300, 33, 1]
+    table, _ = kc.tables([n + 20 for n in lens], 40, 152)
+    state = kc.cache(40, H, D, codes, 153)
+    dev, ref = [t.cuda() for t in state], [t.clone() for t in state]
+    g = torch.Generator().manual_seed(154)
+    mass = torch.zeros(3, H, table.size(1) * 16).cuda()
+    mass64, worst = mass.cpu().double(), 0.0
+    for _ in range(20):
+        k, v, q = (torch.randn(3, n, 1, D, generator=g).bfloat16() for n in (H, H, H * G))
+        fa.append_paged_kv8(k.cuda(), v.cuda(), *dev, table.cuda(), _ints(lens).cuda(), table.size(1))
+        orc.append(k[:, :, 0], v[:, :, 0], *ref, table, _ints(lens))
+        lens = [n + 1 for n in lens]
+        fa.forward_paged_decode_gqa_kv8(q.cuda(), *dev, table.cuda(), _ints(lens).cuda(), table.size(1), mass=mass)
+        out, size = orc.decode(q, *ref, table, lens, mass=mass64)
+        worst = max(worst, kc.decode_bound(q, ref[0], ref[2], out, size, torch.bfloat16, 0.0)[1])
+    # a weight's score and the sum it is divided by, each off by `worst`; 2^-18 for logarithm and exponentials; a rounding of fp32 for each step
+    assert bool(((mass.cpu().double() - mass64).abs() <= mass64 * (2 * worst + 2.0 ** -18 + 20 * 2.0 ** -24)).all())
 
 
 def test_calls_on_another_stream_and_in_a_graph(fa):
