@@ -24,6 +24,7 @@
 // and its codes in turn behind all bytes on their way), more CTAs than fit at once (12 us a wave), keys as they are in three products with whole-numbered
 // parts of q (mma.s8: no conversion, the same time; 37 instead of 32 us for 20 rows of 16 sequences).  Of a step's 2600 cycles 50 are waits for codes and 880
 // the issue of the next copies, which is where a full memory system makes itself felt.
+#include <limits.h>
 #include <math_constants.h>
 
 #include "kv8.cuh"
@@ -487,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
       l[n][0] = l[n][1] = 0.f;
     }
 
-    int spoiled = 0;                            // bit 2n + c: the row has seen a page whose V scale is not finite
+    int spoiled = INT_MAX;                      // first key of the first page whose V scale is not finite
     for (int i = 0; i < x.steps; ++i) {
       const int base = p0 + (turn + share * i) * kTile;
       cp_async_wait<2 * kSlots - 1>();
@@ -498,12 +499,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
         asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(ks[u]), "=f"(vs[u]) : "r"(scales_at + (at_slot * kTile + u) * 8));
         if (!(fabsf(ks[u]) <= 3.4028235e38f)) ks[u] = CUDART_NAN_F;      // a scale that is not finite spoils what sees the page, whatever the codes
         if (base + u >= p1) vs[u] = 0.f;
-        // So does V's, but 0 times it would also spoil what does not see the page: the rows that do are marked, and the page adds nothing.
+        // So does V's, but 0 times it would also spoil what does not see the page: the page adds nothing, and the rows that see it are marked at the end.
         if (!(fabsf(vs[u]) <= 3.4028235e38f)) {
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) spoiled |= (base + u) * kPage < limit[n][c] ? 1 << (n * 2 + c) : 0;
+          spoiled = min(spoiled, (base + u) * kPage);
           vs[u] = 0.f;
         }
       }
@@ -692,14 +690,14 @@ __global__ void __launch_bounds__(kThreads, Shape<D, NT>::kCtas) decode_kernel(c
       at_slot = at_slot + 1 == kSlots ? 0 : at_slot + 1;
     }
 
-    if (spoiled) {
+    if (spoiled != INT_MAX) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int k = 0; k < kSteps; ++k)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (spoiled >> (n * 2 + (e & 1)) & 1) o[n][k][e] = CUDART_NAN_F;
+            if (spoiled < limit[n][e & 1]) o[n][k][e] = CUDART_NAN_F;
     }
     Piece next;
     if (at < end) {                             // the next piece's rows come while this one's go out
