@@ -15,8 +15,8 @@
 // The pages of all sequences and heads are cut evenly over the warps; where there are fewer segments than half the CTAs each is cut into equal
 // parts, at least kLeastPart pages, that the warps of a CTA share.  Parts of a cut segment go through global memory to a second launch, which, like the
 // first, is on its way before the launch in front of it has ended.
-// Measured, int8, 32 heads on 8 of 128: 64 sequences of 512 to 8192 tokens 110.8 us for 573 MB (5.2 TB/s), one of 131071 (e4m3) 51.0 us for 269 MB; four of up to
-// 101 tokens 5.7 us.  Two CTAs of four warps an SM, 16 KB of ring each: with three the first takes as long, the second 57 us (bytes on their way are enough
+// Measured, int8, 32 heads on 8 of 128: 64 sequences of 512 to 8192 tokens 109.9 us for 573 MB (5.2 TB/s), one of 131071 (e4m3) 51.0 us for 269 MB; four of up to
+// 101 tokens 5.8 us.  Two CTAs of four warps an SM, 16 KB of ring each: with three the first takes as long, the second 57 us (bytes on their way are enough
 // with eight warps, and more wait longer for theirs).  Of the first case 4 us pass before the memory is busy and 5 behind the last code; between them it
 // delivers 7.3 TB/s until the first SMs are through, and the last are a sixth later: some get their bytes slower than others.  Looked at and left: loads
 // straight to registers (117), L2 prefetches 2 to 6 steps ahead (slower by 5 to 14 %), a quarter of the pages in small ranges for warps that are through
