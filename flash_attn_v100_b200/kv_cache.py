@@ -430,7 +430,7 @@ class PagedKVCache8(BlockManager):
         rows = before = None
         if mass is not None:
             rows = torch.tensor([self._row[r] for r in request_ids], dtype=torch.int32).to(self.device)
-            if request_ids and (q.size(2) > 1 or any(r in self._guessed for r in request_ids)):
+            if request_ids and (q.size(2) > 1 or self._guessed and any(r in self._guessed for r in request_ids)):
                 before = mass[rows.long(), :, : max(self._tokens[r] for r in request_ids) + q.size(2)]
         out = kv8_ops.forward_paged_decode_gqa_kv8(q, self.k_pools[layer], self.v_pools[layer], self.scales[layer], table, lens,
                                                    self.max_blocks_per_seq, softcap=softcap, mass=mass, mass_index=rows)
@@ -445,6 +445,8 @@ class PagedKVCache8(BlockManager):
         """Blocks and sums of weights as if only the first `kept` (committed by now) of the tokens since the last commit had been there."""
         from . import kv8_ops
         appended, guessed = self._appended.pop(request_id, {}), self._guessed.pop(request_id, {})
+        if not appended and not guessed:
+            return
         row, held = self._row[request_id], self._tokens[request_id] - kept
         table, ints = self.block_table[row: row + 1], lambda v: torch.tensor(v, dtype=torch.int32).to(self.device)
         for layer in sorted({*appended, *guessed}):
